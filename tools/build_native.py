@@ -117,8 +117,11 @@ def _build_host(sources: list[Path], jobs: int, verbose: bool, force: bool) -> P
 def build(jobs: int | None = None, verbose: bool = False, force: bool = False) -> list[Path]:
     jobs = jobs or min(8, os.cpu_count() or 4)
     tlib, tinc, abi = _torch_paths()
+    # packed fp32 instructions stay off: some forms of v_pk_{add,mul,fma}_f32, which -O3 makes from ordinary float
+    # code by itself, give wrong results now and then (the host pass warns that it does not know the feature)
     common = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", f"-I{CSRC / 'include'}",
-              "-Wno-unused-result", "-Wno-deprecated-declarations"]
+              "-Wno-unused-result", "-Wno-deprecated-declarations",
+              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
     torch_flags = [*common, *(f"-I{p}" for p in tinc), f"-I{sysconfig.get_paths()['include']}",
                    f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DUSE_ROCM=1", "-DTORCH_API_INCLUDE_EXTENSION_H"]
     kern_src = sorted((CSRC / "kernels").glob("*.hip")) + [CSRC / "bindings.cpp"]
