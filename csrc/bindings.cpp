@@ -44,6 +44,30 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> dlgm_flash_attn_bwd(const at::Ten
                                                                    const at::Tensor& out, const at::Tensor& lse,
                                                                    double softmax_scale, bool causal,
                                                                    const c10::optional<at::Tensor>& dqkv);
+// shared_attn.hip
+std::tuple<at::Tensor, at::Tensor> dlgm_latent_attn_fwd(const at::Tensor& q, const at::Tensor& kv,
+                                                        const at::Tensor& k_rope, double softmax_scale, bool causal,
+                                                        const c10::optional<at::Tensor>& lens);
+std::tuple<at::Tensor, at::Tensor, at::Tensor> dlgm_latent_attn_bwd(const at::Tensor& dout, const at::Tensor& q,
+                                                                    const at::Tensor& kv, const at::Tensor& k_rope,
+                                                                    const at::Tensor& out, const at::Tensor& lse,
+                                                                    double softmax_scale, bool causal,
+                                                                    const c10::optional<at::Tensor>& lens);
+std::tuple<at::Tensor, at::Tensor> dlgm_prefix_attn_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                        const at::Tensor& prefix_k, const at::Tensor& prefix_v,
+                                                        double softmax_scale, bool causal,
+                                                        const c10::optional<at::Tensor>& lens,
+                                                        const c10::optional<at::Tensor>& prefix_lens);
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> dlgm_prefix_attn_bwd(
+    const at::Tensor& dout, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& prefix_k,
+    const at::Tensor& prefix_v, const at::Tensor& out, const at::Tensor& lse, double softmax_scale, bool causal,
+    const c10::optional<at::Tensor>& lens, const c10::optional<at::Tensor>& prefix_lens);
+// shared_decode.hip
+at::Tensor dlgm_latent_attn_decode(const at::Tensor& q, const at::Tensor& cache, const at::Tensor& lens,
+                                   const at::Tensor& w_kv, double softmax_scale);
+at::Tensor dlgm_prefix_attn_decode(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& lens,
+                                   const at::Tensor& prefix_k, const at::Tensor& prefix_v, double softmax_scale,
+                                   const c10::optional<at::Tensor>& prefix_lens);
 
 // moe.hip
 at::Tensor dlgm_moe_combine_fwd(const at::Tensor& y, const at::Tensor& pos, const c10::optional<at::Tensor>& gates);
@@ -123,6 +147,12 @@ TORCH_LIBRARY(dlgm, m) {
   m.def("transpose_multi(Tensor[] xs, Tensor rows) -> Tensor");
   m.def("transpose(Tensor x, Tensor(a!)? out=None, Tensor? rows=None) -> Tensor");
   m.def("flash_attn_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, float softmax_scale, bool causal, Tensor(a!)? dqkv=None) -> (Tensor, Tensor, Tensor)");
+  m.def("latent_attn_fwd(Tensor q, Tensor kv, Tensor k_rope, float softmax_scale, bool causal, Tensor? lens=None) -> (Tensor, Tensor)");
+  m.def("latent_attn_bwd(Tensor dout, Tensor q, Tensor kv, Tensor k_rope, Tensor out, Tensor lse, float softmax_scale, bool causal, Tensor? lens=None) -> (Tensor, Tensor, Tensor)");
+  m.def("latent_attn_decode(Tensor q, Tensor cache, Tensor lens, Tensor w_kv, float softmax_scale) -> Tensor");
+  m.def("prefix_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor prefix_k, Tensor prefix_v, float softmax_scale, bool causal, Tensor? lens=None, Tensor? prefix_lens=None) -> (Tensor, Tensor)");
+  m.def("prefix_attn_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor prefix_k, Tensor prefix_v, Tensor out, Tensor lse, float softmax_scale, bool causal, Tensor? lens=None, Tensor? prefix_lens=None) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("prefix_attn_decode(Tensor q, Tensor k, Tensor v, Tensor lens, Tensor prefix_k, Tensor prefix_v, float softmax_scale, Tensor? prefix_lens=None) -> Tensor");
   m.def("embedding_fwd(Tensor table, Tensor ids) -> Tensor");
   m.def("embedding_bwd_(Tensor(a!) grad, Tensor dy, Tensor sorted_ids, Tensor order) -> ()");
   m.def("router_topk(Tensor logits, int k) -> (Tensor, Tensor, Tensor)");
@@ -169,6 +199,12 @@ TORCH_LIBRARY_IMPL(dlgm, CUDA, m) {
   m.impl("moe_pad_plan_multi", &dlgm_moe_pad_plan_multi);
   m.impl("transpose_multi", &dlgm_transpose_multi);
   m.impl("transpose", &dlgm_transpose);
+  m.impl("latent_attn_fwd", &dlgm_latent_attn_fwd);
+  m.impl("latent_attn_bwd", &dlgm_latent_attn_bwd);
+  m.impl("latent_attn_decode", &dlgm_latent_attn_decode);
+  m.impl("prefix_attn_fwd", &dlgm_prefix_attn_fwd);
+  m.impl("prefix_attn_bwd", &dlgm_prefix_attn_bwd);
+  m.impl("prefix_attn_decode", &dlgm_prefix_attn_decode);
   m.impl("embedding_fwd", &dlgm_embedding_fwd);
   m.impl("embedding_bwd_", &dlgm_embedding_bwd_);
   m.impl("router_topk", &dlgm_router_topk);

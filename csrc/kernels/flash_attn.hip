@@ -39,139 +39,11 @@
 #include <cstdlib>
 #include <cstring>
 #include <type_traits>
-#include "dlgm_common.h"
+#include "dlgm_attn.h"
 
 using namespace dlgm;
 
 namespace {
-
-typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
-typedef __fp16 hf16x4 __attribute__((ext_vector_type(4)));  // the transpose-read builtin's f16 vector type
-typedef __attribute__((address_space(3))) hf16x4 lds_f16x4;
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-// Deferred rescale (forward): the running max used for exponentiation is only raised when a
-// row's new max exceeds it by more than 2^kRescaleLog2 -- P stays <= 256, exact in fp32 sums.
-constexpr float kRescaleLog2 = 8.f;
-
-// v_exp_f32 as is: exp2f() adds a denormal range fix-up (cmp + cndmask + ldexp per element) that
-// softmax does not need (arguments are <= 0 up to the deferred-rescale slack; underflow -> 0).
-__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// Softmax arithmetic on pairs of accumulator registers. The build keeps packed fp32 instructions off, so a pair is two
-// scalar instructions (forward 0.575 vs 0.574 ms, backward 1.74 vs 1.76 ms at S 8192, 32/8 heads, D 128: the loops do
-// not need the packed forms).
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ f32x2 pk_fma(f32x2 a, f32x2 b, f32x2 c) { return __builtin_elementwise_fma(a, b, c); }
-
-// A condition the caller knows is wave-uniform, made provably so (scalar branch, no exec masking).
-__device__ __forceinline__ bool uniform(bool c) { return __builtin_amdgcn_readfirstlane((int)c) != 0; }
-
-__device__ __forceinline__ f32x16 mfma32(const bf16x8& a, const bf16x8& b, const f32x16& c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-}
-// fp16 compute path (DeepSpeed "fp16" block): the same fragment maps on the f16 MFMA
-__device__ __forceinline__ f32x16 mfma32(const f16x8& a, const f16x8& b, const f32x16& c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-}
-
-// 16-byte-chunk XOR swizzles (see header). D = head dim, rows of D bf16.
-template <int D>
-__device__ __forceinline__ int swz_row(int row, int ch) {  // image read by ds_read_b128 rows
-  if constexpr (D == 128) return ch ^ (row & 15);
-  else return ch ^ ((row >> 1) & 7);
-}
-template <int D>
-__device__ __forceinline__ int swz_tr(int row, int ch) {  // image read by ds_read_b64_tr_b16
-  if constexpr (D == 128) return ch ^ ((row & 3) << 2);
-  else return ch ^ (((row >> 1) & 1) << 2);
-}
-// One image good for both kinds of read (used by the backward's Q / dO / K tiles):
-// plain 256-B rows, chunk ^ (((row&3)<<2) | ((row>>2)&3)); the 128-B-row variant
-// for D = 64 folds the row parity in instead.
-template <int D>
-__device__ __forceinline__ int swz_dual(int row, int ch) {
-  if constexpr (D == 128) return ch ^ (((row & 3) << 2) | ((row >> 2) & 3));
-  else return ch ^ ((((row >> 1) & 1) << 2) | ((row >> 2) & 3));
-}
-
-// Makes x opaque to the optimiser: a per-lane LDS offset computed once before a loop then stays in its
-// register instead of being rebuilt from its row and swizzle parts inside the loop (hipcc re-added
-// them before every read: one v_add_u32 per ds_read in the backward's tile loops).
-__device__ __forceinline__ void pin(int& x) { asm volatile("" : "+v"(x)); }
-
-template <typename E>
-__device__ __forceinline__ vec8_t<E> lds_read_b128(const E* base) {
-  return *reinterpret_cast<const vec8_t<E>*>(base);
-}
-
-// x of lane i ^ 32 (the other half-wave): one v_permlane32_swap instead of an LDS bpermute round trip
-__device__ __forceinline__ float swap_halves(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(__lane_id() < 32 ? r[1] : r[0]);
-}
-
-// Store one 32-row x D accumulator row block (lane (r, h) holds columns 8k + 4h .. +3 of row r for
-// each 8-column group k) as bf16, scaled. One half-exchange (v_permlane32_swap) per dword of a group
-// pair (k, k+1) leaves lanes h = 0 with columns 8k .. 8k+7 and lanes h = 1 with 8k+8 .. 8k+15: one
-// 16-byte store per pair instead of two 8-byte stores (the tail is store-issue bound). Both lanes of
-// a pair share the row, so the swap runs on all lanes and only the store is guarded by `valid`.
-template <int DT, typename E>
-__device__ __forceinline__ void store_rows_bf16(E* row, const f32x16 (&acc)[DT], float scale, int h, bool valid) {
-#pragma unroll
-  for (int k = 0; k < 4 * DT; k += 2) {
-    const f32x16& oa = acc[k >> 2];
-    const f32x16& ob = acc[(k + 1) >> 2];
-    const int ja = 4 * (k & 3), jb = 4 * ((k + 1) & 3);
-    vec4_t<E> va = {(E)(oa[ja] * scale), (E)(oa[ja + 1] * scale), (E)(oa[ja + 2] * scale),
-                    (E)(oa[ja + 3] * scale)};
-    vec4_t<E> vb = {(E)(ob[jb] * scale), (E)(ob[jb + 1] * scale), (E)(ob[jb + 2] * scale),
-                    (E)(ob[jb + 3] * scale)};
-    uint2 a = __builtin_bit_cast(uint2, va), c = __builtin_bit_cast(uint2, vb);
-    const auto sx = __builtin_amdgcn_permlane32_swap(a.x, c.x, false, false);
-    const auto sy = __builtin_amdgcn_permlane32_swap(a.y, c.y, false, false);
-    if (valid) *reinterpret_cast<uint4*>(row + 8 * k + 8 * h) = make_uint4(sx[0], sy[0], sx[1], sy[1]);
-  }
-}
-
-__device__ __forceinline__ bf16x4 lds_read_tr(const bf16* p) {
-  return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(p));
-}
-__device__ __forceinline__ f16x4 lds_read_tr(const f16* p) {
-  return __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_f16x4*)(p)));
-}
-
-__device__ __forceinline__ bf16x8 cat(bf16x4 a, bf16x4 b) {
-  return (bf16x8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-}
-__device__ __forceinline__ f16x8 cat(f16x4 a, f16x4 b) {
-  return (f16x8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-}
-
-typedef __attribute__((address_space(1))) const void* gptr_t;
-typedef __attribute__((address_space(3))) void* lptr_t;
-
-// One LDS-DMA piece: 64 lanes x 16 B = 1 KiB landing lane-linearly at `lds` (wave-uniform).
-__device__ __forceinline__ void glds16(const void* src, void* lds) {
-  __builtin_amdgcn_global_load_lds((gptr_t)src, (lptr_t)lds, 16, 0, 0);
-}
-__device__ __forceinline__ void glds4(const void* src, void* lds) {
-  __builtin_amdgcn_global_load_lds((gptr_t)src, (lptr_t)lds, 4, 0, 0);
-}
-__device__ __forceinline__ void vm_drain() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-
-// One LDS-DMA piece through a buffer descriptor (buffer_load_dwordx4 ... lds): `base` and `nbytes`
-// are wave-uniform (the descriptor lives in SGPRs, reads at or past nbytes return zero), `voff`
-// is the per-lane byte offset, `soff` a wave-uniform byte offset (the tile advance).
-__device__ __forceinline__ void dma16(const void* base, int nbytes, uint32_t voff, uint32_t soff, lptr_t lds) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, nbytes,
-                                                                             0x00020000),
-                                           lds, 16, voff, soff, 0, 0);
-}
-__device__ __forceinline__ void dma16(const void* base, int nbytes, uint32_t voff, uint32_t soff, void* lds) {
-  dma16(base, nbytes, voff, soff, (lptr_t)lds);
-}
 
 // Loop-invariant LDS-DMA plan for a tile of ROWS x D bf16 rows that is re-staged every iteration
 // (the forward's recipe): the per-lane byte offsets of this wave's pieces are computed once, a
@@ -229,12 +101,6 @@ struct TileDma {
     }
   }
 };
-
-// bijective remap of the block id so that consecutive work items land on one XCD
-__device__ __forceinline__ int xcd_remap(int id, int total) {
-  if (total % 8 != 0) return id;
-  return (id % 8) * (total / 8) + id / 8;
-}
 
 template <typename E>
 struct FwdParams {

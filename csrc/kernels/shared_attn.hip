@@ -1,0 +1,789 @@
+// Attention whose keys and values are shared, training forms (gfx950): forward, dQ and dK/dV passes of
+//
+//  * latent attention, expanded: per head h   k[t,h] = [k_nope[t,h] | k_rope[t]],  o = softmax(scale q k^T) v.
+//    k_nope and v are the two halves of ONE up-projected row kv[t,h] (DA + DV wide); k_rope (DB wide) is one vector a
+//    token, shared by the heads -- it is staged beside k_nope as a second LDS image and never copied per head;
+//  * attention over a shared prefix: the B = G n sequences attend to the P prefix keys of their group g = b / n (no
+//    mask, first plen[g] of them) and then causally to their own S keys (first len[b] of them):
+//      o_i = sum_j exp(s_ij) v_j / sum_j exp(s_ij)  over both ranges, one running softmax.
+//
+// Mathematics, all accumulation in fp32:
+//   forward   S^T = K Q^T (query on the lane: row statistics are lane-local), P = exp2(S c - m), O^T += V^T P^T
+//   backward  delta = rowsum(dO * O), P = exp(S - lse), dP = dO V^T, dS = P * (dP - delta),
+//             dQ = scale dS K, dK = scale dS^T Q, dV = P^T dO; dk_rope = sum over heads, d(prefix) = sum over the group's
+//             rows -- fp32 partials summed in a fixed order, no atomics: bits do not depend on scheduling.
+// P and dS are rounded to the 16-bit type before their products: they are matrix-instruction operands.
+//
+// Structure: 4 waves of 32 query rows (forward, dQ) or 32 keys (dK/dV), tiles by LDS-DMA one tile ahead, XOR-swizzled
+// images, transposed operands by ds_read_b64_tr_b16. A tile's descriptor covers exactly its valid rows, so rows past a
+// length read as zero whatever memory holds there (a score is masked besides), and a tile's base is a 64-bit address:
+// no offset of a long sequence passes 32 bits.
+#include <torch/all.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <type_traits>
+#include "dlgm_attn.h"
+#include "dlgm_attn_host.h"
+
+using namespace dlgm;
+
+namespace {
+
+constexpr int kBQ = 128;   // query rows of a forward / dQ workgroup, keys of a dK/dV workgroup
+constexpr int kBKV = 64;   // keys of a forward / dQ tile
+constexpr int kBQ2 = 32;   // queries of a dK/dV tile
+
+template <typename E>
+struct SharedArgs {
+  const E *q, *k, *v, *kr;  // kr: shared rope key [B, S, DB] (latent attention)
+  const E *pk, *pv;         // prefix keys / values [G, P, Hkv, D]
+  const E *o, *dout;        // backward: forward output (contiguous) and its gradient
+  E* out;                   // forward output [B, S, Hq, DV]
+  float* lse;               // [B, Hq, S]
+  float* rows;              // backward [2, B, Hq, S]: -delta, then -lse / scale
+  E* dq;                    // [B, S, Hq, DA + DB]
+  E *dk, *dv, *dpk, *dpv;   // 16-bit gradients of k, v and the prefix (written directly where one part covers them)
+  float *dk_part, *dv_part, *dpk_part, *dpv_part;  // fp32 partials
+  float* dkr_part;          // [Hq, B, S, DB]
+  int64_t q_sb, q_ss, q_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, kr_sb, kr_ss;
+  int64_t pk_sb, pk_ss, pk_sh, pv_sb, pv_ss, pv_sh, do_sb, do_ss, do_sh;
+  int64_t dk_ss, dk_sh, dv_ss, dv_sh;  // row and head strides of dk and dv (batch stride: S rows)
+  const int *lens, *plens;  // [B], [G] valid keys (null: all)
+  int B, S, Hq, Hkv, P, n;  // n: sequences of a group (1 without a prefix)
+  int nsplit;               // dK/dV of a prefix: parts the group's sequences are cut into
+  int prefix_blocks;        // dK/dV workgroups that own prefix keys (they come first)
+  float scale, scale_log2, neg_inv_scale;
+  bool causal;
+
+  __device__ __forceinline__ int len(int b) const { return lens ? min(max(lens[b], 0), S) : S; }
+  __device__ __forceinline__ int plen(int g) const { return plens ? min(max(plens[g], 0), P) : P; }
+};
+
+// ---- forward: one workgroup per (b, q head, 128 queries)
+template <typename E, int DA, int DB, int DV, bool PRE>
+__global__ __launch_bounds__(kThreads, 2) void shared_fwd_kernel(SharedArgs<E> p) {
+  constexpr int KA = DA / 16, KB = DB / 16, KK = KA + KB, DT = DV / 32;
+  constexpr int TA = kBKV * DA, TB = kBKV * DB, TV = kBKV * DV, SLOT = TA + TB + TV;
+  __shared__ __attribute__((aligned(16))) E smem[2 * SLOT];
+
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 31, h = lane >> 5, i16 = lane & 15, g4 = lane >> 4;
+  const int nqt = (p.S + kBQ - 1) / kBQ, group = p.Hq / p.Hkv;
+  // workgroups of one (prefix group, kv head) read the same keys: they follow each other on one XCD, longest first
+  const int work = xcd_remap(blockIdx.x, gridDim.x);
+  const int per_kv = p.n * group * nqt;
+  const int bk = work / per_kv, rem = work - bk * per_kv;
+  const int qt = nqt - 1 - rem / (p.n * group), idx = rem % (p.n * group);
+  const int grp = bk / p.Hkv, hk = bk % p.Hkv, hq = hk * group + idx % group, b = grp * p.n + idx / group;
+
+  const int len = p.len(b);
+  const int q0 = qt * kBQ, q0w = q0 + 32 * w, qcol = q0w + r;
+  const E* qb = p.q + b * p.q_sb + hq * p.q_sh;
+  vec8_t<E> qf[KK];
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) qf[kk] = row8(qb + (int64_t)qcol * p.q_ss + 16 * kk + 8 * h, qcol < len);
+
+  const E* kb = p.k + b * p.k_sb + hk * p.k_sh;
+  const E* vb = p.v + b * p.v_sb + hk * p.v_sh;
+  const E* krb = DB ? p.kr + b * p.kr_sb : nullptr;
+  const E* pkb = PRE ? p.pk + grp * p.pk_sb + hk * p.pk_sh : nullptr;
+  const E* pvb = PRE ? p.pv + grp * p.pv_sb + hk * p.pv_sh : nullptr;
+  const int plen = PRE ? p.plen(grp) : 0;
+  const int np = (plen + kBKV - 1) / kBKV;
+  const int kv_end = p.causal ? min(len, q0 + kBQ) : len;
+  const int nt = q0 < len ? np + (kv_end + kBKV - 1) / kBKV : 0;  // queries past the length have no tile
+
+  const RowTile<E, DA, kBKV, 0> ka(w, lane);
+  const RowTile<E, DB ? DB : 32, kBKV, 0> kr(w, lane);
+  const RowTile<E, DV, kBKV, 2> va(w, lane);
+  auto stage = [&](int buf, int t) {
+    E* img = smem + buf * SLOT;
+    if (PRE && t < np) {
+      const int row0 = t * kBKV;
+      ka.issue(img, pkb + (int64_t)row0 * p.pk_ss, p.pk_ss, plen - row0, w);
+      va.issue(img + TA + TB, pvb + (int64_t)row0 * p.pv_ss, p.pv_ss, plen - row0, w);
+    } else {
+      const int row0 = (t - np) * kBKV;
+      ka.issue(img, kb + (int64_t)row0 * p.k_ss, p.k_ss, len - row0, w);
+      if constexpr (DB > 0) kr.issue(img + TA, krb + (int64_t)row0 * p.kr_ss, p.kr_ss, len - row0, w);
+      va.issue(img + TA + TB, vb + (int64_t)row0 * p.v_ss, p.v_ss, len - row0, w);
+    }
+  };
+
+  f32x16 o[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) o[dt] = (f32x16)(0.f);
+  float m_run = -INFINITY, l_run = 0.f;
+
+  // unrolled by two: the LDS buffer is a compile-time constant in each copy (immediate ds_read offsets)
+  auto tile = [&](auto bufc, int t) {
+    constexpr int buf = decltype(bufc)::value;
+    vm_drain();       // this tile's DMA has landed (this wave's pieces) ...
+    __syncthreads();  // ... and every wave's; the other buffer's readers are done
+    if (t + 1 < nt) stage(buf ^ 1, t + 1);
+    const bool pre = PRE && t < np;
+    const int kv0 = pre ? t * kBKV : (t - np) * kBKV, end = pre ? plen : len;
+    const bool causal = p.causal && !pre;
+    if (causal && kv0 > q0w + 31) return;  // whole tile above this wave's diagonal
+    const E* ki = smem + buf * SLOT;
+    const E* vi = ki + TA + TB;
+    f32x16 s[2] = {(f32x16)(0.f), (f32x16)(0.f)};
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int row = 32 * u + r;
+        const E* a = kk < KA ? ki + row * DA + swz_row<DA>(row, 2 * kk + h) * 8
+                             : ki + TA + row * DB + swz_row<DB ? DB : 32>(row, 2 * (kk - KA) + h) * 8;
+        s[u] = mfma32(lds_read_b128(a), qf[kk], s[u]);
+      }
+    if (uniform((causal && kv0 + kBKV - 1 > q0w) || kv0 + kBKV > end)) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int kv = kv0 + 32 * u + (i & 3) + 8 * (i >> 2) + 4 * h;
+          if (kv >= end || (causal && kv > qcol)) s[u][i] = -INFINITY;
+        }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[u][i]);
+    mx = fmaxf(mx, swap_halves(mx)) * p.scale_log2;
+    if (__any(mx > m_run + kRescaleLog2)) {  // deferred rescale, wave-uniform
+      const float m_new = fmaxf(m_run, mx);
+      const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
+    }
+    const float m_use = m_run == -INFINITY ? 0.f : m_run;
+    vec8_t<E> pf[2][2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float e = fast_exp2(s[u][i] * p.scale_log2 - m_use);
+        s[u][i] = e;
+        l_run += e;
+      }
+      pf[u][0] = pack8<E>(s[u], 0);
+      pf[u][1] = pack8<E>(s[u], 8);
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2)
+          o[dt] = mfma32(read_t<E, DV, 2>(vi, dt, 32 * u + 16 * s2, h, i16, g4), pf[u][s2], o[dt]);
+  };
+  if (nt > 0) stage(0, 0);
+  for (int t = 0; t < nt; t += 2) {
+    tile(std::integral_constant<int, 0>{}, t);
+    if (t + 1 < nt) tile(std::integral_constant<int, 1>{}, t + 1);
+  }
+
+  const float l_tot = l_run + swap_halves(l_run);
+  const bool some = qcol < len && l_tot != 0.f;  // a padded query row: zeros and -inf
+  store_rows_bf16<DT>(p.out + (((int64_t)b * p.S + qcol) * p.Hq + hq) * DV, o, some ? 1.f / l_tot : 0.f, h, qcol < p.S);
+  if (qcol < p.S && h == 0)
+    p.lse[((int64_t)b * p.Hq + hq) * p.S + qcol] = some ? (m_run + log2f(l_tot)) * kLn2 : -INFINITY;
+}
+
+// ---- dQ: one workgroup per (b, q head, 128 queries), the forward's walk. It holds dO in registers, so it also forms
+// delta and writes the [-delta, -lse/scale] rows the dK/dV pass starts its accumulators from (padded rows: 0, 0).
+template <typename E, int DA, int DB, int DV, bool PRE>
+__global__ __launch_bounds__(kThreads, 2) void shared_bwd_dq_kernel(SharedArgs<E> p) {
+  constexpr int KA = DA / 16, KB = DB / 16, KK = KA + KB, KV = DV / 16, DT = (DA + DB) / 32;
+  constexpr int TA = kBKV * DA, TB = kBKV * DB, TV = kBKV * DV, SLOT = TA + TB + TV;
+  constexpr int DBX = DB ? DB : 32;
+  __shared__ __attribute__((aligned(16))) E smem[2 * SLOT];
+
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 31, h = lane >> 5, i16 = lane & 15, g4 = lane >> 4;
+  const int nqt = (p.S + kBQ - 1) / kBQ, group = p.Hq / p.Hkv;
+  const int work = xcd_remap(blockIdx.x, gridDim.x);
+  const int per_kv = p.n * group * nqt;
+  const int bk = work / per_kv, rem = work - bk * per_kv;
+  const int qt = nqt - 1 - rem / (p.n * group), idx = rem % (p.n * group);
+  const int grp = bk / p.Hkv, hk = bk % p.Hkv, hq = hk * group + idx % group, b = grp * p.n + idx / group;
+
+  const int len = p.len(b);
+  const int q0 = qt * kBQ, q0w = q0 + 32 * w, qcol = q0w + r;
+  const bool in = qcol < len;
+  const E* qb = p.q + b * p.q_sb + hq * p.q_sh + (int64_t)qcol * p.q_ss;
+  const E* dob = p.dout + b * p.do_sb + hq * p.do_sh + (int64_t)qcol * p.do_ss;
+  vec8_t<E> qf[KK], dof[KV];
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) qf[kk] = row8(qb + 16 * kk + 8 * h, in);
+#pragma unroll
+  for (int kk = 0; kk < KV; ++kk) dof[kk] = row8(dob + 16 * kk + 8 * h, in);
+  float lse2 = INFINITY, nd = 0.f;
+  {
+    const int64_t rowc = ((int64_t)b * p.Hq + hq) * p.S + qcol;
+    float acc = 0.f;
+    if (in) {
+      const E* orow = p.o + (((int64_t)b * p.S + qcol) * p.Hq + hq) * DV + 8 * h;
+#pragma unroll
+      for (int kk = 0; kk < KV; ++kk) {
+        const vec8_t<E> ov = *reinterpret_cast<const vec8_t<E>*>(orow + 16 * kk);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc += (float)dof[kk][j] * (float)ov[j];
+      }
+      lse2 = p.lse[rowc] * kLog2e;
+    }
+    nd = -(acc + swap_halves(acc));
+    if (qcol < p.S && h == 0) {
+      p.rows[rowc] = nd;
+      p.rows[(int64_t)p.B * p.Hq * p.S + rowc] = in ? p.lse[rowc] * p.neg_inv_scale : 0.f;
+    }
+  }
+
+  const E* kb = p.k + b * p.k_sb + hk * p.k_sh;
+  const E* vb = p.v + b * p.v_sb + hk * p.v_sh;
+  const E* krb = DB ? p.kr + b * p.kr_sb : nullptr;
+  const E* pkb = PRE ? p.pk + grp * p.pk_sb + hk * p.pk_sh : nullptr;
+  const E* pvb = PRE ? p.pv + grp * p.pv_sb + hk * p.pv_sh : nullptr;
+  const int plen = PRE ? p.plen(grp) : 0;
+  const int np = (plen + kBKV - 1) / kBKV;
+  const int kv_end = p.causal ? min(len, q0 + kBQ) : len;
+  const int nt = q0 < len ? np + (kv_end + kBKV - 1) / kBKV : 0;
+
+  const RowTile<E, DA, kBKV, 1> ka(w, lane);
+  const RowTile<E, DBX, kBKV, 1> kr(w, lane);
+  const RowTile<E, DV, kBKV, 0> va(w, lane);
+  auto stage = [&](int buf, int t) {
+    E* img = smem + buf * SLOT;
+    if (PRE && t < np) {
+      const int row0 = t * kBKV;
+      ka.issue(img, pkb + (int64_t)row0 * p.pk_ss, p.pk_ss, plen - row0, w);
+      va.issue(img + TA + TB, pvb + (int64_t)row0 * p.pv_ss, p.pv_ss, plen - row0, w);
+    } else {
+      const int row0 = (t - np) * kBKV;
+      ka.issue(img, kb + (int64_t)row0 * p.k_ss, p.k_ss, len - row0, w);
+      if constexpr (DB > 0) kr.issue(img + TA, krb + (int64_t)row0 * p.kr_ss, p.kr_ss, len - row0, w);
+      va.issue(img + TA + TB, vb + (int64_t)row0 * p.v_ss, p.v_ss, len - row0, w);
+    }
+  };
+
+  f32x16 dqt[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) dqt[dt] = (f32x16)(0.f);
+
+  auto tile = [&](auto bufc, int t) {
+    constexpr int buf = decltype(bufc)::value;
+    vm_drain();
+    __syncthreads();
+    if (t + 1 < nt) stage(buf ^ 1, t + 1);
+    const bool pre = PRE && t < np;
+    const int kv0 = pre ? t * kBKV : (t - np) * kBKV, end = pre ? plen : len;
+    const bool causal = p.causal && !pre;
+    if (causal && kv0 > q0w + 31) return;
+    const E* ki = smem + buf * SLOT;
+    const E* vi = ki + TA + TB;
+    const bool need_mask = uniform((causal && kv0 + kBKV - 1 > q0w) || kv0 + kBKV > end);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {  // one 32-key half at a time: its scores and dP are 32 registers
+      f32x16 s = (f32x16)(0.f), dp = (f32x16)(0.f);
+      const int row = 32 * u + r;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        const E* a = kk < KA ? ki + row * DA + swz_dual<DA>(row, 2 * kk + h) * 8
+                             : ki + TA + row * DB + swz_dual<DBX>(row, 2 * (kk - KA) + h) * 8;
+        s = mfma32(lds_read_b128(a), qf[kk], s);
+        if (kk < KV) dp = mfma32(lds_read_b128(vi + row * DV + swz_row<DV>(row, 2 * kk + h) * 8), dof[kk], dp);
+      }
+      if (need_mask) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int kv = kv0 + 32 * u + (i & 3) + 8 * (i >> 2) + 4 * h;
+          if (kv >= end || (causal && kv > qcol)) s[i] = -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = fast_exp2(s[i] * p.scale_log2 - lse2) * (dp[i] + nd);
+      const vec8_t<E> ds[2] = {pack8<E>(s, 0), pack8<E>(s, 8)};
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2) {
+          const vec8_t<E> a = dt < DA / 32 ? read_t<E, DA, 1>(ki, dt, 32 * u + 16 * s2, h, i16, g4)
+                                           : read_t<E, DBX, 1>(ki + TA, dt - DA / 32, 32 * u + 16 * s2, h, i16, g4);
+          dqt[dt] = mfma32(a, ds[s2], dqt[dt]);
+        }
+    }
+  };
+  if (nt > 0) stage(0, 0);
+  for (int t = 0; t < nt; t += 2) {
+    tile(std::integral_constant<int, 0>{}, t);
+    if (t + 1 < nt) tile(std::integral_constant<int, 1>{}, t + 1);
+  }
+  store_rows_bf16<DT>(p.dq + (((int64_t)b * p.S + qcol) * p.Hq + hq) * (DA + DB), dqt, p.scale, h, qcol < p.S);
+}
+
+// ---- dK / dV: one workgroup per (128 keys, HP q heads of one kv head, a range of sequences). Keys of a sequence are
+// seen by that sequence alone; keys of a prefix by the n sequences of its group, walked one after the other into the
+// same accumulators (cut into nsplit parts where the prefix alone gives too few workgroups).
+template <typename E, int DA, int DB, int DV, bool PRE, int HP>
+__global__ __launch_bounds__(kThreads, DB ? 1 : 2) void shared_bwd_dkdv_kernel(SharedArgs<E> p) {
+  constexpr int KA = DA / 16, KB = DB / 16, KK = KA + KB, KV = DV / 16;
+  constexpr int DTK = (DA + DB) / 32, DTA = DA / 32, DTV = DV / 32;
+  constexpr int DBX = DB ? DB : 32;
+  constexpr int TA = kBQ2 * DA, TB = kBQ2 * DB, TO = kBQ2 * DV, SLOT = TA + TB + TO;
+  __shared__ __attribute__((aligned(16))) E smem[2 * SLOT + kBQ * DV];
+  __shared__ __attribute__((aligned(16))) float rc[2][64];  // [buf][-lse/scale 0..31 | -delta 32..63]
+  E* vimg = smem + 2 * SLOT;
+
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 31, h = lane >> 5, i16 = lane & 15, g4 = lane >> 4;
+  const int group = p.Hq / p.Hkv, nhp = p.Hq / HP;
+  const bool pre = PRE && (int)blockIdx.x < p.prefix_blocks;
+  int b0, b1, hq, k0, part = 0;  // sequences b0 .. b1, first head, first key
+  if (pre) {
+    const int work = xcd_remap(blockIdx.x, p.prefix_blocks);
+    const int nkt = (p.P + kBQ - 1) / kBQ;
+    k0 = work % nkt * kBQ;  // blocks of one (group, part, head pair) share their Q / dO stream
+    int x = work / nkt;
+    hq = x % nhp * HP;
+    x /= nhp;
+    part = x % p.nsplit;
+    const int grp = x / p.nsplit;
+    b0 = grp * p.n + p.n * part / p.nsplit;
+    b1 = grp * p.n + p.n * (part + 1) / p.nsplit;
+  } else {
+    const int id = blockIdx.x - (PRE ? p.prefix_blocks : 0);
+    const int work = xcd_remap(id, gridDim.x - (PRE ? p.prefix_blocks : 0));
+    const int nkt = (p.S + kBQ - 1) / kBQ;
+    k0 = work % nkt * kBQ;  // ascending: most queries first under the causal mask
+    const int x = work / nkt;
+    hq = x % nhp * HP;
+    b0 = x / nhp;
+    b1 = b0 + 1;
+  }
+  const int hk = hq / group, hh = hq % group, grp = b0 / p.n;
+  const int nkeys = pre ? p.plen(grp) : p.len(b0);
+  const bool causal = p.causal && !pre;
+  const int kw0 = k0 + 32 * w, key = kw0 + r;
+  const int64_t k_ss = pre ? p.pk_ss : p.k_ss, v_ss = pre ? p.pv_ss : p.v_ss;
+  const E* kb = pre ? p.pk + grp * p.pk_sb + hk * p.pk_sh : p.k + b0 * p.k_sb + hk * p.k_sh;
+  const E* vb = pre ? p.pv + grp * p.pv_sb + hk * p.pv_sh : p.v + b0 * p.v_sb + hk * p.v_sh;
+
+  // this wave's 32 keys stay in registers (B operand of S = Q K^T); the V rows go to LDS once
+  vec8_t<E> kf[KK];
+#pragma unroll
+  for (int kk = 0; kk < KA; ++kk) kf[kk] = row8(kb + (int64_t)key * k_ss + 16 * kk + 8 * h, key < nkeys);
+  if constexpr (DB > 0) {
+    const E* krb = p.kr + b0 * p.kr_sb + (int64_t)key * p.kr_ss;
+#pragma unroll
+    for (int kk = 0; kk < KB; ++kk) kf[KA + kk] = row8(krb + 16 * kk + 8 * h, key < nkeys);
+  }
+  const RowTile<E, DV, kBQ, 0> vt(w, lane);
+  vt.issue(vimg, vb + (int64_t)k0 * v_ss, v_ss, nkeys - k0, w);
+
+  f32x16 dk[DTK], dv[DTV];  // dK^T, dV^T: [d][key]
+#pragma unroll
+  for (int dt = 0; dt < DTK; ++dt) dk[dt] = (f32x16)(0.f);
+#pragma unroll
+  for (int dt = 0; dt < DTV; ++dt) dv[dt] = (f32x16)(0.f);
+
+  const RowTile<E, DA, kBQ2, 1> qa(w, lane);
+  const RowTile<E, DBX, kBQ2, 1> qr(w, lane);
+  const RowTile<E, DV, kBQ2, 1> da(w, lane);
+  const int64_t nrow = (int64_t)p.B * p.Hq * p.S;
+  // the walk: sequence, head of the pair, 32-query tile (from the diagonal on under the causal mask)
+  const int t0 = causal ? k0 / kBQ2 : 0;
+  struct Cursor {
+    int b, hp, t, nt, len;
+  };
+  auto seek = [&](Cursor& c) {  // the first position at or behind c that has a tile
+    while (c.t >= c.nt) {
+      c.t = t0;
+      if (c.b >= 0 && ++c.hp < HP && t0 < c.nt) return true;
+      c.hp = 0;
+      c.b = c.b < 0 ? b0 : c.b + 1;
+      if (c.b >= b1) return false;
+      c.len = p.len(c.b);
+      c.nt = (c.len + kBQ2 - 1) / kBQ2;
+    }
+    return true;
+  };
+  auto stage = [&](int buf, const Cursor& c) {
+    const int q0 = c.t * kBQ2, hd = hq + c.hp;
+    const E* qb = p.q + c.b * p.q_sb + hd * p.q_sh + (int64_t)q0 * p.q_ss;
+    E* img = smem + buf * SLOT;
+    qa.issue(img, qb, p.q_ss, c.len - q0, w);
+    if constexpr (DB > 0) qr.issue(img + TA, qb + DA, p.q_ss, c.len - q0, w);
+    da.issue(img + TA + TB, p.dout + c.b * p.do_sb + hd * p.do_sh + (int64_t)q0 * p.do_ss, p.do_ss, c.len - q0, w);
+    if (w == 0) {
+      const int q = min(q0 + (lane & 31), p.S - 1);  // rows past the length hold 0, 0 (and are masked)
+      glds4(p.rows + (lane < 32 ? nrow : 0) + ((int64_t)c.b * p.Hq + hd) * p.S + q, &rc[buf][0]);
+    }
+  };
+
+  auto tile = [&](auto bufc, const Cursor& c, bool more, const Cursor& next) {
+    constexpr int buf = decltype(bufc)::value;
+    vm_drain();       // this tile's LDS-DMA has landed ...
+    __syncthreads();  // ... for every wave, and the other buffer's readers are done
+    if (more) stage(buf ^ 1, next);
+    const int q0 = c.t * kBQ2;
+    if (causal && q0 + kBQ2 - 1 < kw0) return;
+    const E* qi = smem + buf * SLOT;
+    const E* di = qi + TA + TB;
+    f32x16 s, dp;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int qr_ = (i & 3) + 8 * (i >> 2) + 4 * h;
+      s[i] = rc[buf][qr_];  // S - lse/scale  ->  P = exp2(that * scale * log2e)
+      dp[i] = rc[buf][32 + qr_];
+    }
+    const int vrow = 32 * w + r;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      const E* a = kk < KA ? qi + r * DA + swz_dual<DA>(r, 2 * kk + h) * 8
+                           : qi + TA + r * DB + swz_dual<DBX>(r, 2 * (kk - KA) + h) * 8;
+      s = mfma32(lds_read_b128(a), kf[kk], s);
+      if (kk < KV)
+        dp = mfma32(lds_read_b128(di + r * DV + swz_dual<DV>(r, 2 * kk + h) * 8),
+                    lds_read_b128(vimg + vrow * DV + swz_row<DV>(vrow, 2 * kk + h) * 8), dp);
+    }
+    if (uniform((causal && q0 < kw0 + 31) || q0 + kBQ2 > c.len || kw0 + 32 > nkeys)) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int q = q0 + (i & 3) + 8 * (i >> 2) + 4 * h;
+        if (key >= nkeys || q >= c.len || (causal && key > q)) s[i] = -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float pv = fast_exp2(s[i] * p.scale_log2);
+      s[i] = pv;
+      dp[i] *= pv;
+    }
+    const vec8_t<E> pf[2] = {pack8<E>(s, 0), pack8<E>(s, 8)}, dsf[2] = {pack8<E>(dp, 0), pack8<E>(dp, 8)};
+#pragma unroll
+    for (int dt = 0; dt < DTK; ++dt)
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2) {
+        if (dt < DTV) dv[dt] = mfma32(read_t<E, DV, 1>(di, dt, 16 * s2, h, i16, g4), pf[s2], dv[dt]);
+        const vec8_t<E> a = dt < DTA ? read_t<E, DA, 1>(qi, dt, 16 * s2, h, i16, g4)
+                                     : read_t<E, DBX, 1>(qi + TA, dt - DTA, 16 * s2, h, i16, g4);
+        dk[dt] = mfma32(a, dsf[s2], dk[dt]);
+      }
+  };
+  static_assert(DTV <= DTK, "the value's columns ride along the key's");
+  Cursor cur{-1, 0, 0, 0, 0};
+  if (k0 < nkeys && seek(cur)) {
+    stage(0, cur);
+    bool more = true;
+    while (more) {
+      Cursor next = cur;
+      ++next.t;
+      more = seek(next);
+      tile(std::integral_constant<int, 0>{}, cur, more, next);
+      if (!more) break;
+      cur = next;
+      ++next.t;
+      more = seek(next);
+      tile(std::integral_constant<int, 1>{}, cur, more, next);
+      cur = next;
+    }
+  }
+  vm_drain();  // a workgroup without a tile still has its V rows in flight
+
+  // rows of this block exist up to `rows`; keys past the length get zeros
+  const int rows = pre ? p.P : p.S;
+  const int nparts = (group / HP) * (pre ? p.nsplit : 1);
+  const int slot = (pre ? part * (group / HP) : 0) + hh / HP;
+  const int64_t base = ((int64_t)(pre ? grp : b0) * rows + key);
+  if constexpr (DB > 0) {  // latent attention: one head owns its k_nope and v rows, the rope part is summed over heads
+    store_rows_bf16<DTA>(p.dk + base * p.dk_ss + hk * p.dk_sh, *reinterpret_cast<f32x16(*)[DTA]>(dk), p.scale, h, key < rows);
+    store_rows_bf16<DTV>(p.dv + base * p.dv_ss + hk * p.dv_sh, dv, 1.f, h, key < rows);
+    if (key < rows)
+      store_rows_f32<DB / 32>(p.dkr_part + (((int64_t)hq * p.B + b0) * p.S + key) * DB, dk + DTA, p.scale, h);
+  } else if (nparts == 1) {
+    E* dkp = pre ? p.dpk : p.dk;
+    E* dvp = pre ? p.dpv : p.dv;
+    store_rows_bf16<DTK>(dkp + (base * p.Hkv + hk) * DA, dk, p.scale, h, key < rows);
+    store_rows_bf16<DTV>(dvp + (base * p.Hkv + hk) * DV, dv, 1.f, h, key < rows);
+  } else if (key < rows) {
+    const int64_t all = (int64_t)(pre ? p.B / p.n : p.B) * rows;  // rows of a part
+    float* dkp = (pre ? p.dpk_part : p.dk_part) + ((slot * all + base) * p.Hkv + hk) * DA;
+    float* dvp = (pre ? p.dpv_part : p.dv_part) + ((slot * all + base) * p.Hkv + hk) * DV;
+    store_rows_f32<DTK>(dkp, dk, p.scale, h);
+    store_rows_f32<DTV>(dvp, dv, 1.f, h);
+  }
+}
+
+// Sum of the fp32 parts in a fixed order -> 16 bits. Up to four tensors in one launch (grid.y).
+template <typename E>
+struct SumArgs {
+  const float* part[4];
+  E* out[4];
+  int64_t n[4];
+  int parts[4];
+};
+template <typename E>
+__global__ __launch_bounds__(256) void sum_parts_kernel(SumArgs<E> a) {
+  const int y = blockIdx.y;
+  const float* part = a.part[y];
+  const int64_t n = a.n[y];
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (int64_t)gridDim.x * 2048) {
+    f32x8 s = (f32x8)(0.f);
+    for (int k = 0; k < a.parts[y]; ++k) s += *reinterpret_cast<const f32x8*>(part + k * n + i);
+    store8f(a.out[y] + i, s);
+  }
+}
+
+// q, kv, k_rope of latent attention: (nope, value) head dims, refused where no kernel is built for them
+std::pair<int, int> check_latent(const at::Tensor& q, const at::Tensor& kv, const at::Tensor& k_rope, const char* op) {
+  check_rows(q, q, op, "q", 4);
+  check_rows(kv, q, op, "kv", 4);
+  check_rows(k_rope, q, op, "k_rope", 3);
+  const int64_t B = q.size(0), S = q.size(1), H = q.size(2);
+  TORCH_CHECK(kv.size(0) == B && kv.size(1) == S && kv.size(2) == H, op, ": kv must be [B, S, H, nope + value]");
+  TORCH_CHECK(k_rope.size(0) == B && k_rope.size(1) == S, op, ": k_rope must be [B, S, rope]");
+  const int64_t dr = k_rope.size(2), dn = q.size(3) - dr, dv = kv.size(3) - dn;
+  TORCH_CHECK((dn == 128 && dr == 64 && dv == 128) || (dn == 64 && dr == 32 && dv == 64), op,
+              ": head dims (nope, rope, value) must be (128, 64, 128) or (64, 32, 64), got (", dn, ", ", dr, ", ", dv, ")");
+  TORCH_CHECK(S < INT32_MAX / 2 && B * H < INT32_MAX, op, ": too many rows");
+  return {(int)dn, (int)dv};
+}
+
+template <typename E>
+SharedArgs<E> latent_args(const at::Tensor& q, const at::Tensor& kv, const at::Tensor& kr, int dn, const int* lens,
+                          double scale, bool causal) {
+  SharedArgs<E> p{};
+  p.q = ptr<E>(q), p.k = ptr<E>(kv), p.v = ptr<E>(kv) + dn, p.kr = ptr<E>(kr);
+  p.q_sb = q.stride(0), p.q_ss = q.stride(1), p.q_sh = q.stride(2);
+  p.k_sb = p.v_sb = kv.stride(0), p.k_ss = p.v_ss = kv.stride(1), p.k_sh = p.v_sh = kv.stride(2);
+  p.kr_sb = kr.stride(0), p.kr_ss = kr.stride(1);
+  p.lens = lens;
+  p.B = q.size(0), p.S = q.size(1), p.Hq = p.Hkv = q.size(2), p.n = 1;
+  p.scale = scale, p.scale_log2 = scale * kLog2e, p.neg_inv_scale = -1.0 / scale;
+  p.causal = causal;
+  return p;
+}
+
+void check_prefix(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& pk,
+                  const at::Tensor& pv, const char* op) {
+  check_rows(q, q, op, "q", 4);
+  check_rows(k, q, op, "k", 4);
+  check_rows(v, q, op, "v", 4);
+  check_rows(pk, q, op, "prefix_k", 4);
+  check_rows(pv, q, op, "prefix_v", 4);
+  const int64_t B = q.size(0), S = q.size(1), Hq = q.size(2), D = q.size(3), Hkv = k.size(2), G = pk.size(0);
+  TORCH_CHECK(D == 64 || D == 128, op, ": head dim must be 64 or 128, got ", D);
+  TORCH_CHECK(k.size(0) == B && k.size(1) == S && k.size(3) == D && v.sizes() == k.sizes(), op,
+              ": k and v must be [B, S, Hkv, D]");
+  TORCH_CHECK(pk.size(2) == Hkv && pk.size(3) == D && pv.sizes() == pk.sizes(), op,
+              ": prefix_k and prefix_v must be [G, P, Hkv, D]");
+  TORCH_CHECK(Hkv > 0 && Hq % Hkv == 0, op, ": q heads must be a multiple of the kv heads");
+  TORCH_CHECK(G > 0 && B % G == 0, op, ": the batch must hold equally many sequences of each prefix");
+  TORCH_CHECK(S < INT32_MAX / 2 && pk.size(1) < INT32_MAX / 2 && B * Hq < INT32_MAX, op, ": too many rows");
+}
+
+template <typename E>
+SharedArgs<E> prefix_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& pk,
+                          const at::Tensor& pv, const int* lens, const int* plens, double scale, bool causal) {
+  SharedArgs<E> p{};
+  p.q = ptr<E>(q), p.k = ptr<E>(k), p.v = ptr<E>(v), p.pk = ptr<E>(pk), p.pv = ptr<E>(pv);
+  p.q_sb = q.stride(0), p.q_ss = q.stride(1), p.q_sh = q.stride(2);
+  p.k_sb = k.stride(0), p.k_ss = k.stride(1), p.k_sh = k.stride(2);
+  p.v_sb = v.stride(0), p.v_ss = v.stride(1), p.v_sh = v.stride(2);
+  p.pk_sb = pk.stride(0), p.pk_ss = pk.stride(1), p.pk_sh = pk.stride(2);
+  p.pv_sb = pv.stride(0), p.pv_ss = pv.stride(1), p.pv_sh = pv.stride(2);
+  p.lens = lens, p.plens = plens;
+  p.B = q.size(0), p.S = q.size(1), p.Hq = q.size(2), p.Hkv = k.size(2), p.P = pk.size(1), p.n = p.B / pk.size(0);
+  p.scale = scale, p.scale_log2 = scale * kLog2e, p.neg_inv_scale = -1.0 / scale;
+  p.causal = causal;
+  return p;
+}
+
+}  // namespace
+
+// q [B, S, H, nope + rope], kv [B, S, H, nope + value], k_rope [B, S, rope] -> out [B, S, H, value], lse [B, H, S]
+std::tuple<at::Tensor, at::Tensor> dlgm_latent_attn_fwd(const at::Tensor& q, const at::Tensor& kv,
+                                                        const at::Tensor& k_rope, double softmax_scale, bool causal,
+                                                        const c10::optional<at::Tensor>& lens) {
+  const char* op = "latent_attn_fwd";
+  const auto [dn, dv] = check_latent(q, kv, k_rope, op);
+  check_scale(softmax_scale, op);
+  const int* lp = check_lens(lens, q, q.size(0), op, "lens");
+  const c10::DeviceGuard guard(q.device());
+  auto out = at::empty({q.size(0), q.size(1), q.size(2), dv}, q.options());
+  auto lse = at::empty({q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
+  if (out.numel() == 0) return {out, lse};
+  const int64_t blocks = check_blocks(q.size(0) * q.size(2) * ((q.size(1) + kBQ - 1) / kBQ), op);
+  auto stream = c10::hip::getCurrentHIPStream();
+  DLGM_DISPATCH_16(q.scalar_type(), E, {
+    auto p = latent_args<E>(q, kv, k_rope, dn, lp, softmax_scale, causal);
+    p.out = ptr<E>(out), p.lse = lse.data_ptr<float>();
+    if (dn == 128) shared_fwd_kernel<E, 128, 64, 128, false><<<blocks, kThreads, 0, stream>>>(p);
+    else shared_fwd_kernel<E, 64, 32, 64, false><<<blocks, kThreads, 0, stream>>>(p);
+  });
+  DLGM_CHECK_HIP(hipGetLastError());
+  return {out, lse};
+}
+
+// Gradients of q, kv and k_rope (contiguous, in their shapes).
+std::tuple<at::Tensor, at::Tensor, at::Tensor> dlgm_latent_attn_bwd(const at::Tensor& dout, const at::Tensor& q,
+                                                                    const at::Tensor& kv, const at::Tensor& k_rope,
+                                                                    const at::Tensor& out, const at::Tensor& lse,
+                                                                    double softmax_scale, bool causal,
+                                                                    const c10::optional<at::Tensor>& lens) {
+  const char* op = "latent_attn_bwd";
+  const auto [dn, dv] = check_latent(q, kv, k_rope, op);
+  check_scale(softmax_scale, op);
+  check_rows(dout, q, op, "dout", 4);
+  check_rows(out, q, op, "out", 4);
+  const int64_t B = q.size(0), S = q.size(1), H = q.size(2), dr = k_rope.size(2);
+  TORCH_CHECK(out.is_contiguous() && out.sizes() == at::IntArrayRef({B, S, H, dv}) && dout.sizes() == out.sizes(), op,
+              ": out must be the contiguous [B, S, H, value] of the forward, dout of its shape");
+  TORCH_CHECK(lse.device() == q.device() && lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
+                  lse.sizes() == at::IntArrayRef({B, H, S}),
+              op, ": lse must be the forward's [B, H, S]");
+  const int* lp = check_lens(lens, q, B, op, "lens");
+  const c10::DeviceGuard guard(q.device());
+  auto dq = at::empty({B, S, H, dn + dr}, q.options());
+  auto dkv = at::empty({B, S, H, dn + dv}, q.options());
+  auto dkr = at::empty({B, S, dr}, q.options());
+  if (B == 0 || S == 0) return {dq, dkv, dkr};
+  if (H == 0) return {dq, dkv, dkr.zero_()};
+  const auto f32 = q.options().dtype(at::kFloat);
+  auto rows = at::empty({2, B, H, S}, f32);
+  auto dkr_part = at::empty({H, B, S, dr}, f32);
+  const int64_t blocks = check_blocks(B * H * ((S + kBQ - 1) / kBQ), op);
+  auto stream = c10::hip::getCurrentHIPStream();
+  DLGM_DISPATCH_16(q.scalar_type(), E, {
+    auto p = latent_args<E>(q, kv, k_rope, dn, lp, softmax_scale, causal);
+    p.o = ptr<E>(out), p.dout = ptr<E>(dout), p.lse = lse.data_ptr<float>(), p.rows = rows.data_ptr<float>();
+    p.do_sb = dout.stride(0), p.do_ss = dout.stride(1), p.do_sh = dout.stride(2);
+    p.dq = ptr<E>(dq), p.dk = ptr<E>(dkv), p.dv = ptr<E>(dkv) + dn;
+    p.dk_ss = p.dv_ss = H * (dn + dv), p.dk_sh = p.dv_sh = dn + dv;
+    p.dkr_part = dkr_part.data_ptr<float>();
+    if (dn == 128) {
+      shared_bwd_dq_kernel<E, 128, 64, 128, false><<<blocks, kThreads, 0, stream>>>(p);
+      shared_bwd_dkdv_kernel<E, 128, 64, 128, false, 1><<<blocks, kThreads, 0, stream>>>(p);
+    } else {
+      shared_bwd_dq_kernel<E, 64, 32, 64, false><<<blocks, kThreads, 0, stream>>>(p);
+      shared_bwd_dkdv_kernel<E, 64, 32, 64, false, 1><<<blocks, kThreads, 0, stream>>>(p);
+    }
+    SumArgs<E> a{};
+    a.part[0] = p.dkr_part, a.out[0] = ptr<E>(dkr), a.n[0] = B * S * dr, a.parts[0] = H;
+    const int64_t grid = std::min<int64_t>((a.n[0] / 8 + 255) / 256, 4096);
+    sum_parts_kernel<E><<<grid, 256, 0, stream>>>(a);
+  });
+  DLGM_CHECK_HIP(hipGetLastError());
+  return {dq, dkv, dkr};
+}
+
+// q [B, S, Hq, D], k/v [B, S, Hkv, D], prefix_k/v [G, P, Hkv, D], B = G n -> out [B, S, Hq, D], lse [B, Hq, S]
+std::tuple<at::Tensor, at::Tensor> dlgm_prefix_attn_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                        const at::Tensor& prefix_k, const at::Tensor& prefix_v,
+                                                        double softmax_scale, bool causal,
+                                                        const c10::optional<at::Tensor>& lens,
+                                                        const c10::optional<at::Tensor>& prefix_lens) {
+  const char* op = "prefix_attn_fwd";
+  check_prefix(q, k, v, prefix_k, prefix_v, op);
+  check_scale(softmax_scale, op);
+  const int* lp = check_lens(lens, q, q.size(0), op, "lens");
+  const int* pp = check_lens(prefix_lens, q, prefix_k.size(0), op, "prefix_lens");
+  const c10::DeviceGuard guard(q.device());
+  auto out = at::empty(q.sizes(), q.options());
+  auto lse = at::empty({q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
+  if (out.numel() == 0) return {out, lse};
+  const int64_t blocks = check_blocks(q.size(0) * q.size(2) * ((q.size(1) + kBQ - 1) / kBQ), op);
+  auto stream = c10::hip::getCurrentHIPStream();
+  DLGM_DISPATCH_16(q.scalar_type(), E, {
+    auto p = prefix_args<E>(q, k, v, prefix_k, prefix_v, lp, pp, softmax_scale, causal);
+    p.out = ptr<E>(out), p.lse = lse.data_ptr<float>();
+    if (q.size(3) == 128) shared_fwd_kernel<E, 128, 0, 128, true><<<blocks, kThreads, 0, stream>>>(p);
+    else shared_fwd_kernel<E, 64, 0, 64, true><<<blocks, kThreads, 0, stream>>>(p);
+  });
+  DLGM_CHECK_HIP(hipGetLastError());
+  return {out, lse};
+}
+
+// Gradients of q, k, v, prefix_k and prefix_v (contiguous, in their shapes).
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> dlgm_prefix_attn_bwd(
+    const at::Tensor& dout, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& prefix_k,
+    const at::Tensor& prefix_v, const at::Tensor& out, const at::Tensor& lse, double softmax_scale, bool causal,
+    const c10::optional<at::Tensor>& lens, const c10::optional<at::Tensor>& prefix_lens) {
+  const char* op = "prefix_attn_bwd";
+  check_prefix(q, k, v, prefix_k, prefix_v, op);
+  check_scale(softmax_scale, op);
+  check_rows(dout, q, op, "dout", 4);
+  check_rows(out, q, op, "out", 4);
+  const int64_t B = q.size(0), S = q.size(1), Hq = q.size(2), D = q.size(3), Hkv = k.size(2);
+  const int64_t G = prefix_k.size(0), P = prefix_k.size(1), n = B / G;
+  TORCH_CHECK(out.is_contiguous() && out.sizes() == q.sizes() && dout.sizes() == q.sizes(), op,
+              ": out must be the contiguous [B, S, Hq, D] of the forward, dout of its shape");
+  TORCH_CHECK(lse.device() == q.device() && lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
+                  lse.sizes() == at::IntArrayRef({B, Hq, S}),
+              op, ": lse must be the forward's [B, Hq, S]");
+  const int* lp = check_lens(lens, q, B, op, "lens");
+  const int* pp = check_lens(prefix_lens, q, G, op, "prefix_lens");
+  const c10::DeviceGuard guard(q.device());
+  auto dq = at::empty(q.sizes(), q.options());
+  auto dk = at::empty(k.sizes(), q.options()), dv = at::empty(k.sizes(), q.options());
+  auto dpk = at::empty(prefix_k.sizes(), q.options()), dpv = at::empty(prefix_k.sizes(), q.options());
+  if (B == 0 || S == 0 || Hq == 0) return {dq.zero_(), dk.zero_(), dv.zero_(), dpk.zero_(), dpv.zero_()};
+  const auto f32 = q.options().dtype(at::kFloat);
+  auto rows = at::empty({2, B, Hq, S}, f32);
+  const int64_t group = Hq / Hkv, hp = group % 2 == 0 ? 2 : 1, gp = group / hp;
+  const int64_t pkt = (P + kBQ - 1) / kBQ;
+  // a group's sequences are cut into parts until the prefix's workgroups fill the chip twice over (256 CUs, two each);
+  // a part costs an fp32 copy of the prefix's gradient, so no more parts than that
+  const int64_t whole = std::max<int64_t>(1, G * (Hq / hp) * pkt);
+  const int64_t nsplit = std::max<int64_t>(1, std::min<int64_t>(n, 1024 / whole));
+  at::Tensor dk_part, dv_part, dpk_part, dpv_part;
+  if (gp > 1) {
+    dk_part = at::empty({gp, B, S, Hkv, D}, f32);
+    dv_part = at::empty({gp, B, S, Hkv, D}, f32);
+  }
+  if (gp * nsplit > 1) {
+    dpk_part = at::empty({gp * nsplit, G, P, Hkv, D}, f32);
+    dpv_part = at::empty({gp * nsplit, G, P, Hkv, D}, f32);
+  }
+  const int64_t q_blocks = check_blocks(B * Hq * ((S + kBQ - 1) / kBQ), op);
+  const int64_t p_blocks = G * (Hq / hp) * nsplit * pkt;
+  const int64_t k_blocks = check_blocks(p_blocks + B * (Hq / hp) * ((S + kBQ - 1) / kBQ), op);
+  auto stream = c10::hip::getCurrentHIPStream();
+  DLGM_DISPATCH_16(q.scalar_type(), E, {
+    auto p = prefix_args<E>(q, k, v, prefix_k, prefix_v, lp, pp, softmax_scale, causal);
+    p.o = ptr<E>(out), p.dout = ptr<E>(dout), p.lse = lse.data_ptr<float>(), p.rows = rows.data_ptr<float>();
+    p.do_sb = dout.stride(0), p.do_ss = dout.stride(1), p.do_sh = dout.stride(2);
+    p.dq = ptr<E>(dq), p.dk = ptr<E>(dk), p.dv = ptr<E>(dv), p.dpk = ptr<E>(dpk), p.dpv = ptr<E>(dpv);
+    p.nsplit = nsplit, p.prefix_blocks = p_blocks;
+    SumArgs<E> a{};
+    int sums = 0;
+    auto sum = [&](const at::Tensor& part, const at::Tensor& to, int64_t parts) {
+      if (!part.defined() || to.numel() == 0) return;
+      a.part[sums] = part.data_ptr<float>(), a.out[sums] = ptr<E>(to), a.n[sums] = to.numel(), a.parts[sums] = parts;
+      ++sums;
+    };
+    sum(dk_part, dk, gp), sum(dv_part, dv, gp), sum(dpk_part, dpk, gp * nsplit), sum(dpv_part, dpv, gp * nsplit);
+    if (gp > 1) p.dk_part = dk_part.data_ptr<float>(), p.dv_part = dv_part.data_ptr<float>();
+    if (gp * nsplit > 1) p.dpk_part = dpk_part.data_ptr<float>(), p.dpv_part = dpv_part.data_ptr<float>();
+    auto run = [&](auto dc) {
+      constexpr int DD = decltype(dc)::value;
+      shared_bwd_dq_kernel<E, DD, 0, DD, true><<<q_blocks, kThreads, 0, stream>>>(p);
+      if (hp == 2) shared_bwd_dkdv_kernel<E, DD, 0, DD, true, 2><<<k_blocks, kThreads, 0, stream>>>(p);
+      else shared_bwd_dkdv_kernel<E, DD, 0, DD, true, 1><<<k_blocks, kThreads, 0, stream>>>(p);
+    };
+    if (D == 128) run(std::integral_constant<int, 128>{});
+    else run(std::integral_constant<int, 64>{});
+    if (sums) {
+      int64_t most = 0;
+      for (int i = 0; i < sums; ++i) most = std::max(most, a.n[i]);
+      const dim3 grid(std::min<int64_t>((most / 8 + 255) / 256, 4096), sums);
+      sum_parts_kernel<E><<<grid, 256, 0, stream>>>(a);
+    }
+  });
+  DLGM_CHECK_HIP(hipGetLastError());
+  return {dq, dk, dv, dpk, dpv};
+}

@@ -1,0 +1,599 @@
+"""Latent attention and attention over a shared prefix, training and single-token forms, against the definition in 64 bits.
+
+Tolerances are elementwise bounds computed beside each expected value (:func:`attend64`). With u = eps / 2 of the type:
+the weights P (and dS) are rounded to the type before their products, so a product with them is off by at most
+u sum |P| |x|; sums run in fp32, an n-term one off by at most n 2^-24 sum |terms|; the result is rounded once more. A score
+that is off by d changes its weight by a factor exp(d). Gradients use delta = rowsum(dO * O) of the ROUNDED output. fp16
+values under 2^-14 have a fixed step: half of it, 2^-25, is added per weight.
+"""
+import math
+
+import pytest
+import torch
+
+from distributed_llm_training_gpu_manager_amd import _native, ops
+
+F32 = 2.0 ** -24
+CPU, GPU = "cpu", "cuda"
+WIDE, HALF = (128, 64, 128), (64, 32, 64)
+
+
+def attend64(q, k, v, ok, scale, dt, do=None):
+    """Attention of q [..., i, d] over k, v [..., j, d] where ok [..., i, j], in 64 bits, and how far a 16-bit
+    implementation may be off BEFORE its last rounding: {name: (value, bound)}."""
+    u = torch.finfo(dt).eps / 2 if dt in (torch.bfloat16, torch.float16) else 0.0
+    sub = 2.0 ** -25 if dt == torch.float16 else 0.0
+    q, k, v = q.double(), k.double(), v.double()
+    d, e, n = q.shape[-1], v.shape[-1], max(q.shape[-2], k.shape[-2])
+    kt, vt = k.transpose(-1, -2), v.transpose(-1, -2)
+    s = (q @ kt) * scale
+    off = (d + 8) * F32 * (q.abs() @ kt.abs()) * scale + 4 * F32 * s.abs()  # of a score
+    off = torch.where(ok, off, 0.0)
+    s = s.masked_fill(~ok, float("-inf"))
+    none = ~ok.any(-1, keepdim=True)
+    m = s.amax(-1, keepdim=True).masked_fill(none, 0.0) if s.shape[-1] else none.double() * 0
+    x = torch.exp(s - m)
+    l = x.sum(-1, keepdim=True)
+    p = x / l.masked_fill(none, 1.0)
+    lse = (m + l.log()).squeeze(-1)
+    top = off.amax(-1, keepdim=True) if s.shape[-1] else none.double() * 0
+    rel = off + top + 2.0 ** -20 + 8 * F32 * lse.abs().masked_fill(none.squeeze(-1), 0.0).unsqueeze(-1)  # of a weight
+    vis = ok.double()
+    out = p @ v
+    res = {"out": (out, (p * (u + rel)) @ v.abs() + (n * F32) * (p @ v.abs()) + sub * (vis @ v.abs())),
+           "lse": (lse, top.squeeze(-1) + 2.0 ** -20 + 8 * F32 * lse.abs().masked_fill(none.squeeze(-1), 0.0))}
+    if do is not None:
+        do = do.double()
+        pt, dot = p.transpose(-1, -2), do.abs()
+        res["dv"] = (pt @ do, (p * (u + rel)).transpose(-1, -2) @ dot + (n * F32) * (pt @ dot) + sub * (vis.transpose(-1, -2) @ dot))
+        dp, delta = do @ vt, (do * out).sum(-1, keepdim=True)
+        dp_off = (e + 8) * F32 * (dot @ vt.abs())
+        delta_off = (dot * (res["out"][1] + u * out.abs() + (e + 8) * F32 * out.abs())).sum(-1, keepdim=True)
+        ds = p * (dp - delta)
+        ds_off = p * (dp_off + delta_off) + ds.abs() * (u + rel + 4 * F32) + sub * vis
+        res["dq"] = ((ds @ k) * scale, scale * (ds_off @ k.abs() + n * F32 * (ds.abs() @ k.abs())))
+        res["dk"] = ((ds.transpose(-1, -2) @ q) * scale,
+                     scale * (ds_off.transpose(-1, -2) @ q.abs() + n * F32 * (ds.abs().transpose(-1, -2) @ q.abs())))
+    return res
+
+
+def close(got, pair, dt, what):
+    """got is within the bound and one rounding of the type."""
+    want, bound = pair
+    u = torch.finfo(dt).eps / 2 if dt in (torch.bfloat16, torch.float16) else 2.0 ** -22
+    tiny = torch.finfo(dt).smallest_normal * u * 2 if dt in (torch.bfloat16, torch.float16) else 0.0
+    got = got.double()
+    assert got.shape == want.shape, what
+    allow = bound * (1 + u) + u * want.abs() + tiny
+    bad = ~((got - want).abs() <= allow) & ~((got == want))
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float(((got - want).abs() - allow)[bad].max()):.3g}"
+
+
+def heads(t):  # [B, S, H, D] -> [B, H, S, D]
+    return t.transpose(1, 2)
+
+
+def group_sum(pair, rep):  # [B, H, S, D] -> [B, H / rep, S, D]
+    return tuple(t.view(t.shape[0], -1, rep, *t.shape[2:]).sum(2) for t in pair)
+
+
+def live(lens, B, S, dev):
+    if lens is None:
+        return torch.ones(B, S, dtype=torch.bool, device=dev)
+    return torch.arange(S, device=dev)[None] < torch.tensor(lens, device=dev)[:, None].clamp(0, S)
+
+
+def rnd(g, *shape, dt, dev, std=1.0):
+    return (torch.randn(*shape, generator=g) * std).to(dt).to(dev)
+
+
+def spoil(t, alive, value=float("nan")):
+    """What lies behind the lengths may hold anything."""
+    t[~alive] = value
+    return t
+
+
+def check_latent(dev, dt, layout, B, S, H, causal=True, lens=None, strided=False, scale=None):
+    dn, dr, dv = layout
+    g = torch.Generator().manual_seed(B * 1000 + S)
+    if strided:  # views of wider rows, the rope key inside the latent projection's row
+        q = rnd(g, B, S, H * (dn + dr) + 16, dt=dt, dev=dev)[..., 16:].unflatten(2, (H, dn + dr))
+        kv = rnd(g, S, B, H + 1, dn + dv, dt=dt, dev=dev).transpose(0, 1)[:, :, 1:]
+        kr = rnd(g, B, S, 64 + dr, dt=dt, dev=dev)[..., 64:]
+        do = rnd(g, B, H, S, dv, dt=dt, dev=dev).transpose(1, 2)
+    else:
+        q, kv = rnd(g, B, S, H, dn + dr, dt=dt, dev=dev), rnd(g, B, S, H, dn + dv, dt=dt, dev=dev)
+        kr, do = rnd(g, B, S, dr, dt=dt, dev=dev), rnd(g, B, S, H, dv, dt=dt, dev=dev)
+    alive = live(lens, B, S, dev)
+    for t in (q, kv, kr, do):
+        spoil(t, alive)
+    lt = None if lens is None else torch.tensor(lens, dtype=torch.int32, device=dev)
+    out, lse = ops.latent_attn_fwd(q, kv, kr, scale, causal, lt)
+    dq, dkv, dkr = ops.latent_attn_bwd(do, q, kv, kr, out, lse, scale, causal, lt)
+    z = lambda t: torch.where(alive.view(B, S, *[1] * (t.dim() - 2)), t.double(), 0.0)  # noqa: E731
+    k = torch.cat([z(kv)[..., :dn], z(kr).unsqueeze(2).expand(B, S, H, dr)], -1)
+    ok = alive[:, None, :] & alive[:, :, None]
+    if causal:
+        ok = ok & torch.ones(S, S, dtype=torch.bool, device=dev).tril()
+    e = attend64(heads(z(q)), heads(k), heads(z(kv)[..., dn:]), ok[:, None].expand(B, H, S, S),
+                 scale or (dn + dr) ** -0.5, dt, heads(z(do)))
+    close(heads(out), e["out"], dt, "out")
+    close(lse, e["lse"], torch.float32, "lse")
+    close(heads(dq), e["dq"], dt, "dq")
+    close(heads(dkv)[..., :dn], tuple(t[..., :dn] for t in e["dk"]), dt, "dk_nope")
+    close(heads(dkv)[..., dn:], e["dv"], dt, "dv")
+    close(dkr, tuple(t[..., dn:].sum(1) for t in e["dk"]), dt, "dk_rope")
+    for t in (out, dq, dkv, dkr):
+        assert not t[~alive].any(), "rows behind a length are zeros"
+
+
+def check_prefix(dev, dt, D, G, n, P, S, Hq, Hkv, causal=True, lens=None, plens=None, strided=False):
+    B, rep = G * n, Hq // Hkv
+    g = torch.Generator().manual_seed(P * 1000 + S)
+    if strided:  # q, k, v as parts of one packed row; the prefix cut from a longer one
+        row = rnd(g, B, S, (Hq + 2 * Hkv) * D, dt=dt, dev=dev)
+        q, k, v = (row[..., a * D:b * D].unflatten(2, (b - a, D)) for a, b in ((0, Hq), (Hq, Hq + Hkv), (Hq + Hkv, Hq + 2 * Hkv)))
+        pk, pv = (rnd(g, G, Hkv, P + 5, D, dt=dt, dev=dev).transpose(1, 2)[:, 5:] for _ in range(2))
+    else:
+        q, k, v = (rnd(g, B, S, h, D, dt=dt, dev=dev) for h in (Hq, Hkv, Hkv))
+        pk, pv = (rnd(g, G, P, Hkv, D, dt=dt, dev=dev) for _ in range(2))
+    do = rnd(g, B, S, Hq, D, dt=dt, dev=dev)
+    alive, palive = live(lens, B, S, dev), live(plens, G, P, dev)
+    for t in (q, k, v, do):
+        spoil(t, alive)
+    for t in (pk, pv):
+        spoil(t, palive, float("inf"))
+    i32 = lambda x: None if x is None else torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    out, lse = ops.prefix_attn_fwd(q, k, v, pk, pv, None, causal, i32(lens), i32(plens))
+    dq, dk, dv, dpk, dpv = ops.prefix_attn_bwd(do, q, k, v, pk, pv, out, lse, None, causal, i32(lens), i32(plens))
+    z = lambda t: torch.where(alive[:, :, None, None], t.double(), 0.0)  # noqa: E731
+    zp = lambda t: torch.where(palive[:, :, None, None], t.double(), 0.0)  # noqa: E731
+    both = lambda a, p: heads(torch.cat([zp(p).repeat_interleave(n, 0), z(a)], 1)).repeat_interleave(rep, 1)  # noqa: E731
+    own = alive[:, None, :] & alive[:, :, None]
+    if causal:
+        own = own & torch.ones(S, S, dtype=torch.bool, device=dev).tril()
+    ok = torch.cat([palive.repeat_interleave(n, 0)[:, None, :] & alive[:, :, None], own], 2)
+    e = attend64(heads(z(q)), both(k, pk), both(v, pv), ok[:, None].expand(B, Hq, S, P + S), D ** -0.5, dt, heads(z(do)))
+    close(heads(out), e["out"], dt, "out")
+    close(lse, e["lse"], torch.float32, "lse")
+    close(heads(dq), e["dq"], dt, "dq")
+    for name, own_g, pre_g in (("dk", dk, dpk), ("dv", dv, dpv)):
+        pair = group_sum(e[name], rep)
+        close(heads(own_g), tuple(t[:, :, P:] for t in pair), dt, name)
+        close(heads(pre_g), tuple(t[:, :, :P].reshape(G, n, Hkv, P, D).sum(1) for t in pair), dt, name + " of the prefix")
+    for t, a in ((out, alive), (dq, alive), (dk, alive), (dv, alive), (dpk, palive), (dpv, palive)):
+        assert not t[~a].any(), "rows behind a length are zeros"
+
+
+def check_latent_decode(dev, dt, layout, r, B, H, L, lens, strided=False):
+    """Four roundings (absorbed query, weights, latent output, result), each off by at most u of what it rounds: 4 u in
+    the 2-norm of a head's output."""
+    dn, dr, dv = layout
+    g = torch.Generator().manual_seed(B * 1000 + L)
+    w = rnd(g, H * (dn + dv), r, dt=dt, dev=dev, std=r ** -0.5)
+    if strided:
+        q = rnd(g, H, B, dn + dr + 8, dt=dt, dev=dev).transpose(0, 1)[..., 8:]
+        cache = rnd(g, L, B, r + dr + 32, dt=dt, dev=dev).transpose(0, 1)[..., :r + dr]
+    else:
+        q, cache = rnd(g, B, H, dn + dr, dt=dt, dev=dev), rnd(g, B, L, r + dr, dt=dt, dev=dev)
+    alive = live(lens, B, L, dev)
+    spoil(cache, alive)
+    out = ops.latent_attention_decode(q, cache, torch.tensor(lens, dtype=torch.int32, device=dev), w)
+    w3, c = w.double().view(H, dn + dv, r), torch.where(alive[..., None], cache.double(), 0.0)
+    kv = torch.einsum("blr,hxr->bhlx", c[..., :r].cpu(), w3.cpu()).to(dev)
+    k = torch.cat([kv[..., :dn], c[:, None, :, r:].expand(B, H, L, dr)], -1)
+    want = attend64(q.double().unsqueeze(2), k, kv[..., dn:], alive[:, None, None, :].expand(B, H, 1, L),
+                    (dn + dr) ** -0.5, dt)["out"][0].squeeze(2)
+    u = torch.finfo(dt).eps / 2 if dt != torch.float32 else 2.0 ** -20
+    err = (out.double() - want).norm(dim=-1)
+    assert (err <= 4 * u * want.norm(dim=-1)).all(), float((err / want.norm(dim=-1).clamp_min(1e-30)).max())
+    assert not out[~alive[:, 0]].any()
+
+
+def check_prefix_decode(dev, dt, D, G, n, P, L, Hq, Hkv, lens, plens=None, strided=False):
+    B, rep = G * n, Hq // Hkv
+    g = torch.Generator().manual_seed(P * 1000 + L)
+    q = rnd(g, Hq, B, D, dt=dt, dev=dev).transpose(0, 1) if strided else rnd(g, B, Hq, D, dt=dt, dev=dev)
+    if strided:
+        k, v = (rnd(g, B, Hkv, L, D, dt=dt, dev=dev).transpose(1, 2) for _ in range(2))
+        pk, pv = (rnd(g, P, G, Hkv, D + 8, dt=dt, dev=dev).transpose(0, 1)[..., :D] for _ in range(2))
+    else:
+        k, v = (rnd(g, B, L, Hkv, D, dt=dt, dev=dev) for _ in range(2))
+        pk, pv = (rnd(g, G, P, Hkv, D, dt=dt, dev=dev) for _ in range(2))
+    alive, palive = live(lens, B, L, dev), live(plens, G, P, dev)
+    for t in (k, v):
+        spoil(t, alive)
+    for t in (pk, pv):
+        spoil(t, palive)
+    i32 = lambda x: None if x is None else torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    out = ops.prefix_attention_decode(q, k, v, i32(lens), pk, pv, i32(plens))
+    z = lambda t, a: torch.where(a[:, :, None, None], t.double(), 0.0)  # noqa: E731
+    both = lambda a, p: heads(torch.cat([z(p, palive).repeat_interleave(n, 0), z(a, alive)], 1)).repeat_interleave(rep, 1)  # noqa: E731
+    ok = torch.cat([palive.repeat_interleave(n, 0), alive], 1)
+    e = attend64(q.double().unsqueeze(2), both(k, pk), both(v, pv), ok[:, None, None, :].expand(B, Hq, 1, P + L), D ** -0.5, dt)
+    close(out, tuple(t.squeeze(2) for t in e["out"]), dt, "out")
+    assert not out[~ok.any(1)].any()
+
+
+# ---- the reference path (CPU) ------------------------------------------------------------------
+
+def test_reference_latent():
+    for causal in (True, False):
+        check_latent(CPU, torch.float32, HALF, 3, 17, 3, causal, [17, 0, 5])
+    check_latent(CPU, torch.float32, (16, 8, 24), 1, 9, 2, strided=True)
+
+
+def test_reference_prefix():
+    check_prefix(CPU, torch.float32, 16, 2, 2, 7, 9, 4, 2, True, [9, 0, 1, 4], [7, 3])
+    check_prefix(CPU, torch.float32, 16, 1, 3, 0, 5, 3, 3, False, [5, 0, 2], strided=True)
+
+
+def test_reference_decode():
+    check_latent_decode(CPU, torch.float32, (16, 8, 24), 32, 3, 5, 11, [11, 0, 1])
+    check_prefix_decode(CPU, torch.float32, 16, 2, 2, 7, 9, 4, 2, [9, 0, 0, 4], [7, 0])
+
+
+@pytest.mark.parametrize("lens", [None, [4, 2]])
+def test_gradients_match_differences(lens):
+    """The differentiable entry points against finite differences in 64 bits."""
+    g = torch.Generator().manual_seed(0)
+    x = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64, requires_grad=True)  # noqa: E731
+    lt = None if lens is None else torch.tensor(lens, dtype=torch.int32)
+    assert torch.autograd.gradcheck(lambda *a: ops.latent_attention(*a, lens=lt), (x(2, 4, 2, 5), x(2, 4, 6), x(2, 4, 2), x(2 * 7, 6)))
+    assert torch.autograd.gradcheck(lambda *a: ops.prefix_attention(*a, lens=lt),
+                                    (x(2, 4, 4, 3), x(2, 4, 2, 3), x(2, 4, 2, 3), x(1, 3, 2, 3), x(1, 3, 2, 3)))
+
+
+def test_absorbed_and_expanded_agree():
+    """The last token of the expanded form is the absorbed form over the cache of all tokens."""
+    g = torch.Generator().manual_seed(1)
+    B, S, H, dn, dr, dv, r = 2, 6, 3, 8, 4, 5, 16
+    q, c, kr = (torch.randn(*s, generator=g, dtype=torch.float64) for s in ((B, S, H, dn + dr), (B, S, r), (B, S, dr)))
+    w = torch.randn(H * (dn + dv), r, generator=g, dtype=torch.float64)
+    a = ops.latent_attention(q, c, kr, w)[:, -1]
+    b = ops.latent_attention_decode(q[:, -1], torch.cat([c, kr], -1), torch.full((B,), S, dtype=torch.int32), w)
+    assert torch.allclose(a, b, rtol=1e-12, atol=1e-12)
+
+
+def _latent_args(dev, dt=torch.bfloat16, B=2, S=8, H=2, layout=HALF):
+    dn, dr, dv = layout
+    g = torch.Generator().manual_seed(0)
+    return [rnd(g, *s, dt=dt, dev=dev) for s in ((B, S, H, dn + dr), (B, S, H, dn + dv), (B, S, dr))]
+
+
+@pytest.mark.parametrize("dev", [CPU, pytest.param(GPU, marks=pytest.mark.gpu)])
+def test_shapes_that_do_not_fit_are_refused(dev):
+    q, kv, kr = _latent_args(dev)
+    c, w = torch.zeros(2, 8, 16, dtype=q.dtype, device=dev), torch.zeros(2 * 128, 16, dtype=q.dtype, device=dev)
+    for bad in ((q, c[:, :4], kr, w), (q, c, kr[:1], w), (q, c, kr, w[:, :8]), (q, c, kr, w[:-1]), (q, c, kr, w[:64])):
+        with pytest.raises(ValueError):
+            ops.latent_attention(*bad)
+    k = torch.zeros(6, 8, 2, 64, dtype=q.dtype, device=dev)
+    qq, pk = torch.zeros(6, 8, 4, 64, dtype=q.dtype, device=dev), torch.zeros(4, 3, 2, 64, dtype=q.dtype, device=dev)
+    for args in ((qq, k, k, pk, pk), (qq, k, k, pk[:2, :, :1], pk[:2, :, :1]), (qq[:, :, :3], k, k, pk[:2], pk[:2]), (qq, k, k, pk[:0], pk[:0])):
+        with pytest.raises(ValueError):
+            ops.prefix_attention(*args)
+        with pytest.raises(ValueError):
+            ops.prefix_attention_decode(args[0][:, 0], *args[1:3], torch.zeros(6, dtype=torch.int32, device=dev), *args[3:])
+
+
+# ---- the kernels (GPU) -------------------------------------------------------------------------
+
+BF, FP = torch.bfloat16, torch.float16
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,layout,B,S,H,causal,lens,strided", [
+    (BF, WIDE, 1, 1, 1, True, None, False),
+    (BF, WIDE, 2, 128, 2, True, None, False),
+    (FP, WIDE, 3, 129, 3, True, [129, 0, 64], False),
+    (BF, WIDE, 2, 333, 2, False, [333, 1], True),
+    (FP, WIDE, 1, 511, 5, False, None, False),
+    (BF, HALF, 2, 63, 3, True, None, True),
+    (FP, HALF, 4, 200, 2, True, [1, 200, 31, 97], False),
+    (BF, HALF, 2, 65, 1, False, [65, 33], True),
+    (FP, HALF, 1, 640, 9, True, None, False),
+])
+def test_latent_kernels(dt, layout, B, S, H, causal, lens, strided):
+    check_latent(GPU, dt, layout, B, S, H, causal, lens, strided)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,D,G,n,P,S,Hq,Hkv,causal,lens,plens,strided", [
+    (BF, 128, 1, 1, 1, 1, 1, 1, True, None, None, False),
+    (BF, 128, 1, 4, 256, 128, 8, 2, True, None, None, False),
+    (FP, 128, 2, 2, 130, 65, 4, 4, True, [65, 0, 7, 64], [130, 63], True),
+    (BF, 128, 1, 3, 0, 200, 6, 2, True, [200, 1, 128], None, False),
+    (FP, 128, 3, 1, 77, 33, 3, 1, False, [33, 0, 5], [0, 77, 1], False),
+    (BF, 64, 2, 3, 300, 40, 4, 2, True, None, [300, 129], True),
+    (FP, 64, 1, 5, 64, 129, 12, 12, True, [129, 64, 0, 1, 100], None, False),
+    (BF, 64, 1, 2, 513, 17, 6, 1, False, None, [0], False),
+    (FP, 64, 1, 8, 1000, 3, 2, 2, True, None, None, False),
+])
+def test_prefix_kernels(dt, D, G, n, P, S, Hq, Hkv, causal, lens, plens, strided):
+    check_prefix(GPU, dt, D, G, n, P, S, Hq, Hkv, causal, lens, plens, strided)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,layout,r,B,H,L,lens,strided", [
+    (BF, WIDE, 512, 1, 1, 1, [1], False),
+    (BF, WIDE, 512, 3, 32, 300, [300, 0, 64], False),
+    (FP, WIDE, 512, 2, 65, 129, [129, 65], True),
+    (FP, WIDE, 256, 5, 8, 1000, [1000, 999, 63, 1, 0], False),
+    (BF, WIDE, 256, 33, 2, 70, [70 - 2 * i for i in range(33)], True),
+    (BF, HALF, 512, 2, 20, 513, [500, 513], False),
+    (FP, HALF, 256, 1, 130, 4100, [4100], False),
+    (BF, HALF, 256, 40, 3, 5, [i % 6 for i in range(40)], False),
+])
+def test_latent_decode_kernel(dt, layout, r, B, H, L, lens, strided):
+    check_latent_decode(GPU, dt, layout, r, B, H, L, lens, strided)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,D,G,n,P,L,Hq,Hkv,lens,plens,strided", [
+    (BF, 128, 1, 1, 1, 1, 1, 1, [0], None, False),
+    (BF, 128, 1, 4, 500, 60, 8, 8, [60, 1, 0, 33], None, False),
+    (FP, 128, 2, 17, 300, 129, 8, 2, [129 - 4 * i % 130 for i in range(34)], [300, 0], False),
+    (BF, 128, 1, 40, 1500, 20, 8, 2, [i % 21 for i in range(40)], [1401], True),
+    (FP, 128, 1, 3, 0, 260, 40, 1, [260, 0, 128], None, False),
+    (BF, 64, 3, 2, 127, 0, 6, 2, [0] * 6, [127, 0, 128], False),
+    (FP, 64, 1, 6, 9000, 300, 12, 12, [300, 299, 0, 1, 128, 127], None, True),
+    (BF, 64, 2, 2, 64, 1000, 70, 1, [1000, 5, 0, 640], [0, 64], False),
+])
+def test_prefix_decode_kernel(dt, D, G, n, P, L, Hq, Hkv, lens, plens, strided):
+    check_prefix_decode(GPU, dt, D, G, n, P, L, Hq, Hkv, lens, plens, strided)
+
+
+def _train_inputs(seed, dev=GPU, dt=BF):
+    g = torch.Generator().manual_seed(seed)
+    B, S, H, (dn, dr, dv), r = 2, 150, 4, WIDE, 256
+    q, c, kr = (rnd(g, *s, dt=dt, dev=dev) for s in ((B, S, H, dn + dr), (B, S, r), (B, S, dr)))
+    w, do = rnd(g, H * (dn + dv), r, dt=dt, dev=dev, std=r ** -0.5), rnd(g, B, S, H, dv, dt=dt, dev=dev)
+    return q, c, kr, w, do
+
+
+@pytest.mark.gpu
+def test_latent_attention_is_its_parts():
+    """The differentiable entry point is the GEMM, the kernel pair and the GEMMs of the backward, bit for bit; its values and
+    gradients are those of the CPU reference up to the roundings on the way (up-projection, weights, output, and in a
+    gradient two more: at most 6 u in the 2-norm)."""
+    q, c, kr, w, do = _train_inputs(0)
+    lens = torch.tensor([150, 77], dtype=torch.int32, device=GPU)
+    leaves = [t.clone().requires_grad_(True) for t in (q, c, kr, w)]
+    out = ops.latent_attention(*leaves, lens=lens)
+    grads = torch.autograd.grad(out, leaves, do)
+    kv = (c.view(300, -1) @ w.t()).view(2, 150, 4, -1)
+    o, lse = ops.latent_attn_fwd(q, kv, kr, lens=lens)
+    dq, dkv, dkr = ops.latent_attn_bwd(do, q, kv, kr, o, lse, lens=lens)
+    assert torch.equal(out, o) and torch.equal(grads[0], dq) and torch.equal(grads[2], dkr)
+    ref = [t.cpu().double().requires_grad_(True) for t in (q, c, kr, w)]
+    ro = ops.latent_attention(*ref, lens=lens.cpu())
+    rg = torch.autograd.grad(ro, ref, do.cpu().double())
+    u = torch.finfo(BF).eps / 2
+    for a, b in zip((out, *grads), (ro, *rg)):
+        assert float((a.cpu().double() - b).norm()) <= 6 * u * float(b.norm())
+
+
+@pytest.mark.gpu
+def test_training_and_sampling_of_a_group():
+    """As used together: answers sampled token by token over a shared prefix get the outputs that the training form gives
+    the whole answers, and the same for a latent cache."""
+    g = torch.Generator().manual_seed(3)
+    G, n, P, S, Hq, Hkv, D, dt = 1, 3, 200, 20, 4, 2, 128, BF
+    q, k, v = (rnd(g, G * n, S, h, D, dt=dt, dev=GPU) for h in (Hq, Hkv, Hkv))
+    pk, pv = (rnd(g, G, P, Hkv, D, dt=dt, dev=GPU) for _ in range(2))
+    whole = ops.prefix_attention(q, k, v, pk, pv)
+    u = torch.finfo(dt).eps / 2
+    for t in (0, 7, S - 1):
+        one = ops.prefix_attention_decode(q[:, t], k, v, torch.full((n,), t + 1, dtype=torch.int32, device=GPU), pk, pv)
+        # both are within their own bound of the exact value: two roundings of each side, at most 4 u of sum p |v|
+        assert float((one - whole[:, t]).abs().max()) <= 4 * u * float(v.abs().max())
+    q, c, kr, w, _ = _train_inputs(4)
+    whole = ops.latent_attention(q, c, kr, w)
+    cache = torch.cat([c, kr], -1)
+    for t in (0, 63, 149):
+        one = ops.latent_attention_decode(q[:, t], cache, torch.full((2,), t + 1, dtype=torch.int32, device=GPU), w)
+        # seven roundings between the two (kv, weights, output; absorbed query, weights, latent output, output)
+        err = (one.double() - whole[:, t].double()).norm()
+        assert float(err) <= 7 * u * float(whole[:, t].double().norm())
+
+
+@pytest.mark.gpu
+def test_same_inputs_same_bits():
+    g = torch.Generator().manual_seed(5)
+    q, k, v, do = (rnd(g, 6, 70, h, 64, dt=BF, dev=GPU) for h in (8, 2, 2, 8))
+    pk, pv = (rnd(g, 2, 300, 2, 64, dt=BF, dev=GPU) for _ in range(2))
+
+    def once():
+        out, lse = ops.prefix_attn_fwd(q, k, v, pk, pv)
+        lens = torch.full((6,), 70, dtype=torch.int32, device=GPU)
+        return (out, lse, *ops.prefix_attn_bwd(do, q, k, v, pk, pv, out, lse),
+                ops.prefix_attention_decode(q[:, 0], k, v, lens, pk, pv))
+
+    a, b = once(), once()
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.gpu
+def test_captured_graphs_replay():
+    """Both training pairs and both single-token forms captured into two graphs, replayed on new inputs with eager work
+    between the replays; every replay equals the eager result."""
+    q, c, kr, w, do = _train_inputs(6)
+    kv = (c.view(300, -1) @ w.t()).view(2, 150, 4, -1)
+    cache = torch.cat([c, kr], -1)
+    lens = torch.tensor([150, 33], dtype=torch.int32, device=GPU)
+    g = torch.Generator().manual_seed(7)
+    pq, pk_, pv_, pdo = (rnd(g, 4, 50, h, 64, dt=BF, dev=GPU) for h in (4, 2, 2, 4))
+    xk, xv = (rnd(g, 1, 190, 2, 64, dt=BF, dev=GPU) for _ in range(2))
+    plens = torch.tensor([50, 3, 0, 20], dtype=torch.int32, device=GPU)
+
+    def latent():
+        out, lse = ops.latent_attn_fwd(q, kv, kr, lens=lens)
+        return (out, *ops.latent_attn_bwd(do, q, kv, kr, out, lse, lens=lens), ops.latent_attention_decode(q[:, 0], cache, lens, w))
+
+    def prefix():
+        out, lse = ops.prefix_attn_fwd(pq, pk_, pv_, xk, xv, lens=plens)
+        return (out, *ops.prefix_attn_bwd(pdo, pq, pk_, pv_, xk, xv, out, lse, lens=plens),
+                ops.prefix_attention_decode(pq[:, 0], pk_, pv_, plens, xk, xv))
+
+    graphs = []
+    for fn in (latent, prefix):
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            fn()
+        torch.cuda.current_stream().wait_stream(s)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs = fn()
+        graphs.append((gr, outs, fn))
+    for i in range(4):
+        for t in (q, kv, kr, do, cache, pq, pk_, pv_, pdo, xk, xv):
+            t.mul_(0.9 + 0.1 * i)
+        lens[1] = 33 + i
+        plens[2] = i
+        for gr, _, _ in graphs:
+            gr.replay()
+        want = [fn() for _, _, fn in graphs]
+        torch.cuda.synchronize()
+        for (_, outs, _), ws in zip(graphs, want):
+            assert all(torch.equal(a, b) for a, b in zip(outs, ws)), f"replay {i}"
+
+
+@pytest.mark.gpu
+def test_runs_on_the_current_stream():
+    """Inputs made on a side stream and used there, without any synchronisation with the default stream."""
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        q, kv, kr = _latent_args(GPU, S=300)
+        out, lse = ops.latent_attn_fwd(q, kv, kr)
+        grads = ops.latent_attn_bwd(torch.ones_like(out), q, kv, kr, out, lse)
+    s.synchronize()
+    out2, lse2 = ops.latent_attn_fwd(q, kv, kr)
+    grads2 = ops.latent_attn_bwd(torch.ones_like(out), q, kv, kr, out2, lse2)
+    assert torch.equal(out, out2) and all(torch.equal(a, b) for a, b in zip(grads, grads2))
+
+
+@pytest.mark.gpu
+def test_rows_beyond_32_bit_offsets():
+    """Row strides and cache lengths whose byte offsets pass 32 bits."""
+    dn, dr, dv = HALF
+    g = torch.Generator().manual_seed(8)
+    S, H = 520, 2
+    buf = torch.empty(S, 1 << 22, dtype=BF, device=GPU)  # 4.4 GB
+    kv = buf[:, -H * (dn + dv):].view(1, S, H, dn + dv)
+    kv.copy_(rnd(g, 1, S, H, dn + dv, dt=BF, dev=GPU))
+    q, kr, do = (rnd(g, *s, dt=BF, dev=GPU) for s in ((1, S, H, dn + dr), (1, S, dr), (1, S, H, dv)))
+    out, lse = ops.latent_attn_fwd(q, kv, kr)
+    a = (out, *ops.latent_attn_bwd(do, q, kv, kr, out, lse))
+    out2, lse2 = ops.latent_attn_fwd(q, kv.contiguous(), kr)
+    b = (out2, *ops.latent_attn_bwd(do, q, kv.contiguous(), kr, out2, lse2))
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    del buf, kv
+    # a cache of 3.9 million tokens, 4.5 GB: zeros but for the last 40, which a scaled query picks out
+    r, L, n = 512, 3_900_000, 40
+    w = rnd(g, H * (dn + dv), r, dt=BF, dev=GPU, std=r ** -0.5)
+    cache = torch.zeros(1, L, r + dr, dtype=BF, device=GPU)
+    cache[:, -n:] = rnd(g, 1, n, r + dr, dt=BF, dev=GPU)
+    q = rnd(g, 1, H, dn + dr, dt=BF, dev=GPU) * 8
+    got = ops.latent_attention_decode(q, cache, torch.tensor([L], dtype=torch.int32, device=GPU), w).double()
+    w3, c = w.double().view(H, dn + dv, r), cache[0, -n:].double()
+    for h in range(H):
+        s = (c[:, :r] @ (w3[h, :dn].t() @ q[0, h, :dn].double()) + c[:, r:] @ q[0, h, dn:].double()) * (dn + dr) ** -0.5
+        e = torch.exp(s)
+        want = w3[h, dn:] @ ((e / (e.sum() + (L - n))) @ c[:, :r])
+        # the absorbed query's rounding moves a score by at most u sum |qa| |c| scale
+        qa = (w3[h, :dn].t() @ q[0, h, :dn].double()).abs()
+        u = torch.finfo(BF).eps / 2
+        off = float((c[:, :r].abs() @ qa).max()) * u * (dn + dr) ** -0.5
+        assert float((got[0, h] - want).norm()) <= (3 * u + math.expm1(2 * off)) * float(want.norm())
+
+
+@pytest.mark.gpu
+def test_kernels_refuse_what_they_cannot_do():
+    q, kv, kr = _latent_args(GPU)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=GPU)  # noqa: E731
+    out, lse = ops.latent_attn_fwd(q, kv, kr)
+    bad = [
+        lambda: ops.latent_attn_fwd(q.float(), kv.float(), kr.float()),
+        lambda: ops.latent_attn_fwd(q.half(), kv, kr),
+        lambda: ops.latent_attn_fwd(q, kv[:1], kr),
+        lambda: ops.latent_attn_fwd(q, kv[..., :96], kr),
+        lambda: ops.latent_attn_fwd(q, kv, kr[..., :16]),
+        lambda: ops.latent_attn_fwd(q, kv.cpu(), kr),
+        lambda: ops.latent_attn_fwd(q, kv, kr, lens=i32(8, 8).long()),
+        lambda: ops.latent_attn_fwd(q, kv, kr, lens=i32(8)),
+        lambda: ops.latent_attn_fwd(q, kv, kr, lens=i32(8, 8).cpu()),
+        lambda: ops.latent_attn_fwd(q, kv, kr, softmax_scale=0.0),
+        lambda: ops.latent_attn_fwd(q, kv, kr, softmax_scale=float("nan")),
+        lambda: ops.latent_attn_fwd(q.transpose(2, 3), kv, kr),
+        lambda: ops.latent_attn_fwd(torch.zeros(2, 8, 2, 97, dtype=BF, device=GPU)[..., 1:], kv, kr),
+        lambda: ops.latent_attn_bwd(out[:1], q, kv, kr, out, lse),
+        lambda: ops.latent_attn_bwd(out, q, kv, kr, out, lse.double()),
+        lambda: ops.latent_attn_bwd(out, q, kv, kr, out.transpose(1, 2).contiguous().transpose(1, 2), lse),
+    ]
+    cache, w = torch.zeros(2, 9, 256 + 32, dtype=BF, device=GPU), torch.zeros(2 * 128, 256, dtype=BF, device=GPU)
+    one = q[:, 0]
+    bad += [
+        lambda: ops.latent_attention_decode(one, cache, i32(1, 2), w[:, :248]),
+        lambda: ops.latent_attention_decode(one, cache, i32(1, 2), w[:-1]),
+        lambda: ops.latent_attention_decode(one, cache[:1], i32(1, 2), w),
+        lambda: ops.latent_attention_decode(one, cache, i32(1), w),
+        lambda: ops.latent_attention_decode(one, cache.half(), i32(1, 2), w),
+        lambda: ops.latent_attention_decode(one, cache[..., :-1], i32(1, 2), w),
+    ]
+    pq, k, pk = (torch.zeros(*s, dtype=BF, device=GPU) for s in ((4, 8, 4, 64), (4, 8, 2, 64), (2, 5, 2, 64)))
+    bad += [
+        lambda: ops.prefix_attn_fwd(pq[..., :32], k[..., :32], k[..., :32], pk[..., :32], pk[..., :32]),
+        lambda: ops.prefix_attn_fwd(pq, k, k[:, :4], pk, pk),
+        lambda: ops.prefix_attn_fwd(pq, k, k, pk, pk[:, :4]),
+        lambda: ops.prefix_attn_fwd(pq, k, k, pk, pk, prefix_lens=i32(1, 2, 3)),
+        lambda: ops.prefix_attn_fwd(pq, k.half(), k.half(), pk, pk),
+        lambda: ops.prefix_attention_decode(pq[:, 0], k, k, i32(1, 2, 3), pk, pk),
+        lambda: ops.prefix_attention_decode(pq[:, 0], k, k[:3], i32(1, 2, 3, 4), pk, pk),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises((RuntimeError, ValueError, NotImplementedError)):
+            call()
+            pytest.fail(f"call {i} was not refused")
+
+
+@pytest.mark.gpu
+def test_empty_tensors():
+    q, kv, kr = _latent_args(GPU)
+    out, lse = ops.latent_attn_fwd(q[:0], kv[:0], kr[:0])
+    assert out.shape == (0, 8, 2, 64) and all(t.numel() == 0 for t in ops.latent_attn_bwd(out, q[:0], kv[:0], kr[:0], out, lse))
+    out, lse = ops.latent_attn_fwd(q[:, :0], kv[:, :0], kr[:, :0])
+    assert out.shape == (2, 0, 2, 64)
+    cache, w = torch.zeros(2, 0, 288, dtype=BF, device=GPU), torch.zeros(256, 256, dtype=BF, device=GPU)
+    assert not ops.latent_attention_decode(q[:, 0], cache, torch.zeros(2, dtype=torch.int32, device=GPU), w).any()
+    pq, k, pk = (torch.zeros(*s, dtype=BF, device=GPU) for s in ((2, 0, 4, 64), (2, 0, 2, 64), (1, 5, 2, 64)))
+    out, lse = ops.prefix_attn_fwd(pq, k, k, pk, pk)
+    g = ops.prefix_attn_bwd(out, pq, k, k, pk, pk, out, lse)
+    assert g[3].shape == pk.shape and not g[3].any() and not g[4].any()
+    none = ops.prefix_attention_decode(torch.ones(2, 4, 64, dtype=BF, device=GPU), k, k, torch.zeros(2, dtype=torch.int32, device=GPU), pk[:, :0], pk[:, :0])
+    assert none.shape == (2, 4, 64) and not none.any()
+
+
+@pytest.mark.gpu
+def test_nan_reaches_the_output():
+    """A NaN in a live row is a NaN in what depends on it (the NaN trap sees it), never a zero."""
+    q, kv, kr = _latent_args(GPU, S=70)
+    kv[0, 3, 0, 0] = float("nan")
+    out, _ = ops.latent_attn_fwd(q, kv, kr)
+    assert out[0, 3:, 0].isnan().all() and not out[0, :, 1].isnan().any() and not out[1].isnan().any()
+    cache, w = torch.ones(2, 70, 288, dtype=BF, device=GPU), torch.ones(256, 256, dtype=BF, device=GPU)
+    cache[0, 5, 7] = float("nan")
+    o = ops.latent_attention_decode(q[:, 0] * 0.01, cache, torch.tensor([70, 70], dtype=torch.int32, device=GPU), w * 0.01)
+    assert o[0].isnan().all() and not o[1].isnan().any()
+    k = torch.ones(2, 9, 2, 64, dtype=BF, device=GPU)
+    pk = k[:1].clone()
+    k[1, 2, 1, 5] = float("nan")
+    qq = torch.ones(2, 4, 64, dtype=BF, device=GPU)
+    o = ops.prefix_attention_decode(qq, k, k.nan_to_num(), torch.tensor([9, 9], dtype=torch.int32, device=GPU), pk, pk)
+    assert o[1, 2:].isnan().all() and not o[1, :2].isnan().any() and not o[0].isnan().any()
+
+
+@pytest.mark.gpu
+def test_native_kernels_are_registered():
+    assert _native.hip_available() and hasattr(torch.ops.dlgm, "latent_attn_decode") and hasattr(torch.ops.dlgm, "prefix_attn_bwd")
