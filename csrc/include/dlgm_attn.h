@@ -182,16 +182,32 @@ __device__ __forceinline__ vec8_t<E> row8(const E* p, bool ok) {
   return ok ? *reinterpret_cast<const vec8_t<E>*>(p) : (vec8_t<E>)((E)0.f);
 }
 
-// A operand (32 columns dt of rows r1, r1 + 8 per lane group) read transposed from an image of D-wide rows
-template <typename E, int D, int SWZ>
-__device__ __forceinline__ vec8_t<E> read_t(const E* img, int dt, int row0, int h, int i16, int g) {
-  const int col = dt * 32 + 16 * (g & 1) + 4 * (i16 & 3);
-  const int ch = col >> 3, within = col & 7;
-  const int r1 = row0 + 4 * h + (i16 >> 2), r2 = r1 + 8;
-  const int c1 = SWZ == 2 ? swz_tr<D>(r1, ch) : swz_dual<D>(r1, ch);
-  const int c2 = SWZ == 2 ? swz_tr<D>(r2, ch) : swz_dual<D>(r2, ch);
-  return cat(lds_read_tr(img + r1 * D + c1 * 8 + within), lds_read_tr(img + r2 * D + c2 * 8 + within));
-}
+// Where a lane reads its fragments in an image of D-wide rows (element offsets). All swizzles XOR the 16-byte chunk of a
+// row, whose bits lie below the row's, so every fragment is one lane offset XOR a constant plus an immediate. A loop pins
+// the offset once an iteration: left to itself the compiler keeps one register per fragment (some 30 in the wide backward,
+// which then spilled 49: dQ 2296 us at S 8192, 32 heads).
+template <int D, int SWZ>  // SWZ: 0 row image, 1 dual image
+struct RowFrag {           // row `r` of a 32-row block, 8 columns 16 kk + 8 h
+  int at;
+  __device__ __forceinline__ RowFrag(int r, int h) {
+    at = r * D + ((SWZ ? swz_dual<D>(r, h) : swz_row<D>(r, h)) << 3);
+  }
+  __device__ __forceinline__ int operator()(int kk) const { return at ^ (kk << 4); }
+};
+template <int D, int SWZ>  // SWZ: 1 dual image, 2 transposed-read image
+struct TrFrag {            // columns 32 dt .. +31 of rows row0 + {4 h .. +3, 8 + 4 h .. +3}, transposed: an A operand
+  int at;
+  __device__ __forceinline__ TrFrag(int h, int i16, int g) {
+    const int col = 16 * (g & 1) + 4 * (i16 & 3), row = 4 * h + (i16 >> 2), ch = col >> 3;
+    at = row * D + ((SWZ == 2 ? swz_tr<D>(row, ch) : swz_dual<D>(row, ch)) << 3) + (col & 7);
+  }
+  template <typename E>
+  __device__ __forceinline__ vec8_t<E> read(const E* img, int dt, int row0) const {
+    constexpr int X = SWZ == 1 || D == 32 ? 16 : 0;  // how the swizzle of row + 8 differs
+    const int a = at ^ (dt << 5);
+    return cat(lds_read_tr(img + row0 * D + a), lds_read_tr(img + (row0 + 8) * D + (a ^ X)));
+  }
+};
 
 // fp32 rows of a transposed accumulator: lane (key r, half h) holds columns 8k + 4h .. +3
 template <int DT>

@@ -64,6 +64,7 @@ template <typename E, int DA, int DB, int DV, bool PRE>
 __global__ __launch_bounds__(kThreads, 2) void shared_fwd_kernel(SharedArgs<E> p) {
   constexpr int KA = DA / 16, KB = DB / 16, KK = KA + KB, DT = DV / 32;
   constexpr int TA = kBKV * DA, TB = kBKV * DB, TV = kBKV * DV, SLOT = TA + TB + TV;
+  constexpr int DBX = DB ? DB : 32;
   __shared__ __attribute__((aligned(16))) E smem[2 * SLOT];
 
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -94,7 +95,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_fwd_kernel(SharedArgs<E> p
   const int nt = q0 < len ? np + (kv_end + kBKV - 1) / kBKV : 0;  // queries past the length have no tile
 
   const RowTile<E, DA, kBKV, 0> ka(w, lane);
-  const RowTile<E, DB ? DB : 32, kBKV, 0> kr(w, lane);
+  const RowTile<E, DBX, kBKV, 0> kr(w, lane);
   const RowTile<E, DV, kBKV, 2> va(w, lane);
   auto stage = [&](int buf, int t) {
     E* img = smem + buf * SLOT;
@@ -114,6 +115,9 @@ __global__ __launch_bounds__(kThreads, 2) void shared_fwd_kernel(SharedArgs<E> p
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) o[dt] = (f32x16)(0.f);
   float m_run = -INFINITY, l_run = 0.f;
+  RowFrag<DA, 0> kf(r, h);
+  RowFrag<DBX, 0> krf(r, h);
+  TrFrag<DV, 2> vf(h, i16, g4);
 
   // unrolled by two: the LDS buffer is a compile-time constant in each copy (immediate ds_read offsets)
   auto tile = [&](auto bufc, int t) {
@@ -132,9 +136,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_fwd_kernel(SharedArgs<E> p
     for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int row = 32 * u + r;
-        const E* a = kk < KA ? ki + row * DA + swz_row<DA>(row, 2 * kk + h) * 8
-                             : ki + TA + row * DB + swz_row<DB ? DB : 32>(row, 2 * (kk - KA) + h) * 8;
+        const E* a = kk < KA ? ki + 32 * u * DA + kf(kk) : ki + TA + 32 * u * DB + krf(kk - KA);
         s[u] = mfma32(lds_read_b128(a), qf[kk], s[u]);
       }
     if (uniform((causal && kv0 + kBKV - 1 > q0w) || kv0 + kBKV > end)) {
@@ -179,7 +181,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_fwd_kernel(SharedArgs<E> p
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2)
-          o[dt] = mfma32(read_t<E, DV, 2>(vi, dt, 32 * u + 16 * s2, h, i16, g4), pf[u][s2], o[dt]);
+          o[dt] = mfma32(vf.read(vi, dt, 32 * u + 16 * s2), pf[u][s2], o[dt]);
   };
   if (nt > 0) stage(0, 0);
   for (int t = 0; t < nt; t += 2) {
@@ -273,6 +275,11 @@ __global__ __launch_bounds__(kThreads, 2) void shared_bwd_dq_kernel(SharedArgs<E
   f32x16 dqt[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) dqt[dt] = (f32x16)(0.f);
+  RowFrag<DA, 1> kf(r, h);
+  RowFrag<DBX, 1> krf(r, h);
+  RowFrag<DV, 0> vf(r, h);
+  TrFrag<DA, 1> kt(h, i16, g4);
+  TrFrag<DBX, 1> krt(h, i16, g4);
 
   auto tile = [&](auto bufc, int t) {
     constexpr int buf = decltype(bufc)::value;
@@ -289,13 +296,13 @@ __global__ __launch_bounds__(kThreads, 2) void shared_bwd_dq_kernel(SharedArgs<E
 #pragma unroll
     for (int u = 0; u < 2; ++u) {  // one 32-key half at a time: its scores and dP are 32 registers
       f32x16 s = (f32x16)(0.f), dp = (f32x16)(0.f);
-      const int row = 32 * u + r;
+      pin(kf.at), pin(vf.at), pin(kt.at);
+      if constexpr (DB > 0) pin(krf.at), pin(krt.at);
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
-        const E* a = kk < KA ? ki + row * DA + swz_dual<DA>(row, 2 * kk + h) * 8
-                             : ki + TA + row * DB + swz_dual<DBX>(row, 2 * (kk - KA) + h) * 8;
+        const E* a = kk < KA ? ki + 32 * u * DA + kf(kk) : ki + TA + 32 * u * DB + krf(kk - KA);
         s = mfma32(lds_read_b128(a), qf[kk], s);
-        if (kk < KV) dp = mfma32(lds_read_b128(vi + row * DV + swz_row<DV>(row, 2 * kk + h) * 8), dof[kk], dp);
+        if (kk < KV) dp = mfma32(lds_read_b128(vi + 32 * u * DV + vf(kk)), dof[kk], dp);
       }
       if (need_mask) {
 #pragma unroll
@@ -311,8 +318,8 @@ __global__ __launch_bounds__(kThreads, 2) void shared_bwd_dq_kernel(SharedArgs<E
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2) {
-          const vec8_t<E> a = dt < DA / 32 ? read_t<E, DA, 1>(ki, dt, 32 * u + 16 * s2, h, i16, g4)
-                                           : read_t<E, DBX, 1>(ki + TA, dt - DA / 32, 32 * u + 16 * s2, h, i16, g4);
+          const vec8_t<E> a = dt < DA / 32 ? kt.read(ki, dt, 32 * u + 16 * s2)
+                                           : krt.read(ki + TA, dt - DA / 32, 32 * u + 16 * s2);
           dqt[dt] = mfma32(a, ds[s2], dqt[dt]);
         }
     }
@@ -390,6 +397,13 @@ __global__ __launch_bounds__(kThreads, DB ? 1 : 2) void shared_bwd_dkdv_kernel(S
 #pragma unroll
   for (int dt = 0; dt < DTV; ++dt) dv[dt] = (f32x16)(0.f);
 
+  RowFrag<DA, 1> qf(r, h);
+  RowFrag<DBX, 1> qrf(r, h);
+  RowFrag<DV, 1> df(r, h);
+  RowFrag<DV, 0> vf(r, h);
+  TrFrag<DA, 1> qt(h, i16, g4);
+  TrFrag<DBX, 1> qrt(h, i16, g4);
+  TrFrag<DV, 1> dt_(h, i16, g4);
   const RowTile<E, DA, kBQ2, 1> qa(w, lane);
   const RowTile<E, DBX, kBQ2, 1> qr(w, lane);
   const RowTile<E, DV, kBQ2, 1> da(w, lane);
@@ -440,15 +454,11 @@ __global__ __launch_bounds__(kThreads, DB ? 1 : 2) void shared_bwd_dkdv_kernel(S
       s[i] = rc[buf][qr_];  // S - lse/scale  ->  P = exp2(that * scale * log2e)
       dp[i] = rc[buf][32 + qr_];
     }
-    const int vrow = 32 * w + r;
+    const E* vi = vimg + 32 * w * DV;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
-      const E* a = kk < KA ? qi + r * DA + swz_dual<DA>(r, 2 * kk + h) * 8
-                           : qi + TA + r * DB + swz_dual<DBX>(r, 2 * (kk - KA) + h) * 8;
-      s = mfma32(lds_read_b128(a), kf[kk], s);
-      if (kk < KV)
-        dp = mfma32(lds_read_b128(di + r * DV + swz_dual<DV>(r, 2 * kk + h) * 8),
-                    lds_read_b128(vimg + vrow * DV + swz_row<DV>(vrow, 2 * kk + h) * 8), dp);
+      s = mfma32(lds_read_b128(kk < KA ? qi + qf(kk) : qi + TA + qrf(kk - KA)), kf[kk], s);
+      if (kk < KV) dp = mfma32(lds_read_b128(di + df(kk)), lds_read_b128(vi + vf(kk)), dp);
     }
     if (uniform((causal && q0 < kw0 + 31) || q0 + kBQ2 > c.len || kw0 + 32 > nkeys)) {
 #pragma unroll
@@ -468,9 +478,8 @@ __global__ __launch_bounds__(kThreads, DB ? 1 : 2) void shared_bwd_dkdv_kernel(S
     for (int dt = 0; dt < DTK; ++dt)
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2) {
-        if (dt < DTV) dv[dt] = mfma32(read_t<E, DV, 1>(di, dt, 16 * s2, h, i16, g4), pf[s2], dv[dt]);
-        const vec8_t<E> a = dt < DTA ? read_t<E, DA, 1>(qi, dt, 16 * s2, h, i16, g4)
-                                     : read_t<E, DBX, 1>(qi + TA, dt - DTA, 16 * s2, h, i16, g4);
+        if (dt < DTV) dv[dt] = mfma32(dt_.read(di, dt, 16 * s2), pf[s2], dv[dt]);
+        const vec8_t<E> a = dt < DTA ? qt.read(qi, dt, 16 * s2) : qrt.read(qi + TA, dt - DTA, 16 * s2);
         dk[dt] = mfma32(a, dsf[s2], dk[dt]);
       }
   };

@@ -55,9 +55,10 @@ __global__ __launch_bounds__(kThreads) void latent_absorb_kernel(LatentArgs<E> p
   wt.issue(img, p.w + (int64_t)head * (p.dn + p.dv) * p.w_ss + c0, p.w_ss, DN, w);
   vm_drain();
   __syncthreads();
+  const TrFrag<128, 2> wf(h, i16, g4);
   vec8_t<E> a[DN / 16];
 #pragma unroll
-  for (int s = 0; s < DN / 16; ++s) a[s] = read_t<E, 128, 2>(img, w, 16 * s, h, i16, g4);
+  for (int s = 0; s < DN / 16; ++s) a[s] = wf.read(img, w, 16 * s);
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const int b = b0 + r;
     const E* q = p.q + b * p.q_sb + head * p.q_sh;
@@ -122,6 +123,9 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attend_kernel(LatentArgs<E
   for (int x = 0; x < 2; ++x)
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[x][dt] = (f32x16)(0.f);
+  RowFrag<128, 1> cf(r, h);
+  RowFrag<DR, 0> rf(r, h);
+  TrFrag<128, 1> vf(h, i16, g4);
   float m_run[2] = {-INFINITY, -INFINITY}, l_run = 0.f;  // maxima of heads r and 32 + r; the sum of this wave's rows
 
   auto tile = [&](auto bufc, int t) {
@@ -130,12 +134,11 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attend_kernel(LatentArgs<E
     __syncthreads();
     if (t + 1 < t1) stage(buf ^ 1, t + 1);
     const E* img = smem + buf * SLOT;
-    const int row = 32 * u + r;
+    pin(cf.at), pin(rf.at), pin(vf.at);
     f32x16 s = (f32x16)(0.f);
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
-      const E* a = kk < KR ? img + kk / 8 * TI + row * 128 + swz_dual<128>(row, 2 * (kk % 8) + h) * 8
-                           : img + NI * TI + row * DR + swz_row<DR>(row, 2 * (kk - KR) + h) * 8;
+      const E* a = kk < KR ? img + kk / 8 * TI + 32 * u * 128 + cf(kk % 8) : img + NI * TI + 32 * u * DR + rf(kk - KR);
       s = mfma32(lds_read_b128(a), qf[kk], s);
     }
     if (uniform(t * 64 + 64 > len)) {
@@ -186,7 +189,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attend_kernel(LatentArgs<E
       const E* vi = img + col / 4 * TI;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const vec8_t<E> a = read_t<E, 128, 1>(vi, col % 4, 16 * k, h, i16, g4);
+        const vec8_t<E> a = vf.read(vi, col % 4, 16 * k);
         o[0][dt] = mfma32(a, pf[0][k], o[0][dt]);
         o[1][dt] = mfma32(a, pf[1][k], o[1][dt]);
       }
@@ -335,6 +338,8 @@ __global__ __launch_bounds__(kThreads, 1) void prefix_attend_kernel(PrefixArgs<E
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) o[dt] = (f32x16)(0.f);
   float m_run = -INFINITY, l_run = 0.f;
+  const RowFrag<D, 0> kf(r, h);
+  const TrFrag<D, 2> vf(h, i16, g4);
   if (t0 < t1) stage(0, t0);
   for (int t = t0; t < t1; ++t) {
     vm_drain();
@@ -348,7 +353,7 @@ __global__ __launch_bounds__(kThreads, 1) void prefix_attend_kernel(PrefixArgs<E
       const E* vi = ki + TI;
       f32x16 s = (f32x16)(0.f);
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) s = mfma32(lds_read_b128(ki + r * D + swz_row<D>(r, 2 * kk + h) * 8), qf[kk], s);
+      for (int kk = 0; kk < KK; ++kk) s = mfma32(lds_read_b128(ki + kf(kk)), qf[kk], s);
       if (uniform(key0 + 32 > len)) {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
@@ -376,7 +381,7 @@ __global__ __launch_bounds__(kThreads, 1) void prefix_attend_kernel(PrefixArgs<E
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int s2 = 0; s2 < 2; ++s2) o[dt] = mfma32(read_t<E, D, 2>(vi, dt, 16 * s2, h, i16, g4), pf[s2], o[dt]);
+        for (int s2 = 0; s2 < 2; ++s2) o[dt] = mfma32(vf.read(vi, dt, 16 * s2), pf[s2], o[dt]);
     }
   }
 
