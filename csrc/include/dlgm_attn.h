@@ -124,6 +124,11 @@ __device__ __forceinline__ void glds4(const void* src, void* lds) {
   __builtin_amdgcn_global_load_lds((gptr_t)src, (lptr_t)lds, 4, 0, 0);
 }
 __device__ __forceinline__ void vm_drain() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// all but this wave's N youngest vector-memory operations are done
+template <int N>
+__device__ __forceinline__ void vm_wait() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
 
 // One LDS-DMA piece through a buffer descriptor (buffer_load_dwordx4 ... lds): `base` and `nbytes`
 // are wave-uniform (the descriptor lives in SGPRs, reads at or past nbytes return zero), `voff`
@@ -153,12 +158,12 @@ struct RowTile {
   static_assert((NW * PR) % 16 == 0, "piece step must be a multiple of the swizzle period");
   int row, col;  // this lane's row of the first piece, its source byte in the row
   __device__ __forceinline__ RowTile(int wave, int lane) {
-    row = wave * PR + lane / CH;
+    row = wave % NP * PR + lane / CH;
     const int phys = lane % CH;
     col = 16 * (SWZ == 2 ? swz_tr<D>(row, phys) : SWZ == 1 ? swz_dual<D>(row, phys) : swz_row<D>(row, phys));
   }
   __device__ __forceinline__ void issue(E* img, const E* base, int64_t stride, int valid, int wave) const {
-    if (NP < NW && wave >= NP) return;
+    if (NP < NW) wave %= NP;  // fewer pieces than waves: some load one twice, so every wave issues PPW loads
     const int bytes = valid > 0 ? (int)((int64_t)(min(valid, ROWS) - 1) * stride * 2) + D * 2 : 0;
     const uint32_t step = (uint32_t)(stride * 2);
     uint32_t off = (uint32_t)row * step + col;

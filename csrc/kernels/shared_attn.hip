@@ -31,7 +31,9 @@ namespace {
 
 constexpr int kBQ = 128;   // query rows of a forward / dQ workgroup, keys of a dK/dV workgroup
 constexpr int kBKV = 64;   // keys of a forward / dQ tile
-constexpr int kBQ2 = 32;   // queries of a dK/dV tile
+constexpr int kBQP = 32;   // queries of a dK/dV tile over a prefix ...
+constexpr int kBQ2 = 64;   // ... and of latent attention
+constexpr int kKvThreads = 512;
 
 template <typename E>
 struct SharedArgs {
@@ -332,23 +334,23 @@ __global__ __launch_bounds__(kThreads, 2) void shared_bwd_dq_kernel(SharedArgs<E
   store_rows_bf16<DT>(p.dq + (((int64_t)b * p.S + qcol) * p.Hq + hq) * (DA + DB), dqt, p.scale, h, qcol < p.S);
 }
 
-// ---- dK / dV: one workgroup per (128 keys, HP q heads of one kv head, a range of sequences). Keys of a sequence are
+// ---- dK / dV over a shared prefix: one workgroup per (128 keys, HP q heads of one kv head, a range of sequences). Keys of a sequence are
 // seen by that sequence alone; keys of a prefix by the n sequences of its group, walked one after the other into the
 // same accumulators (cut into nsplit parts where the prefix alone gives too few workgroups).
-template <typename E, int DA, int DB, int DV, bool PRE, int HP>
-__global__ __launch_bounds__(kThreads, DB ? 1 : 2) void shared_bwd_dkdv_kernel(SharedArgs<E> p) {
-  constexpr int KA = DA / 16, KB = DB / 16, KK = KA + KB, KV = DV / 16;
-  constexpr int DTK = (DA + DB) / 32, DTA = DA / 32, DTV = DV / 32;
-  constexpr int DBX = DB ? DB : 32;
-  constexpr int TA = kBQ2 * DA, TB = kBQ2 * DB, TO = kBQ2 * DV, SLOT = TA + TB + TO;
-  __shared__ __attribute__((aligned(16))) E smem[2 * SLOT + kBQ * DV];
+// A wave of 32 keys keeps K and the gradients in registers and V in LDS: two waves a SIMD. (The split of the latent kernel
+// below, two waves to 32 keys, measured 1622 us here against 1306 at 8 x 1024 queries over 4096 + 1024 keys, 32/8 heads.)
+template <typename E, int D, int HP>
+__global__ __launch_bounds__(kThreads, 2) void prefix_bwd_dkdv_kernel(SharedArgs<E> p) {
+  constexpr int KK = D / 16, DT = D / 32;
+  constexpr int TA = kBQP * D, SLOT = 2 * TA;
+  __shared__ __attribute__((aligned(16))) E smem[2 * SLOT + kBQ * D];
   __shared__ __attribute__((aligned(16))) float rc[2][64];  // [buf][-lse/scale 0..31 | -delta 32..63]
   E* vimg = smem + 2 * SLOT;
 
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 31, h = lane >> 5, i16 = lane & 15, g4 = lane >> 4;
   const int group = p.Hq / p.Hkv, nhp = p.Hq / HP;
-  const bool pre = PRE && (int)blockIdx.x < p.prefix_blocks;
+  const bool pre = (int)blockIdx.x < p.prefix_blocks;
   int b0, b1, hq, k0, part = 0;  // sequences b0 .. b1, first head, first key
   if (pre) {
     const int work = xcd_remap(blockIdx.x, p.prefix_blocks);
@@ -362,8 +364,8 @@ __global__ __launch_bounds__(kThreads, DB ? 1 : 2) void shared_bwd_dkdv_kernel(S
     b0 = grp * p.n + p.n * part / p.nsplit;
     b1 = grp * p.n + p.n * (part + 1) / p.nsplit;
   } else {
-    const int id = blockIdx.x - (PRE ? p.prefix_blocks : 0);
-    const int work = xcd_remap(id, gridDim.x - (PRE ? p.prefix_blocks : 0));
+    const int id = blockIdx.x - p.prefix_blocks;
+    const int work = xcd_remap(id, gridDim.x - p.prefix_blocks);
     const int nkt = (p.S + kBQ - 1) / kBQ;
     k0 = work % nkt * kBQ;  // ascending: most queries first under the causal mask
     const int x = work / nkt;
@@ -382,34 +384,21 @@ __global__ __launch_bounds__(kThreads, DB ? 1 : 2) void shared_bwd_dkdv_kernel(S
   // this wave's 32 keys stay in registers (B operand of S = Q K^T); the V rows go to LDS once
   vec8_t<E> kf[KK];
 #pragma unroll
-  for (int kk = 0; kk < KA; ++kk) kf[kk] = row8(kb + (int64_t)key * k_ss + 16 * kk + 8 * h, key < nkeys);
-  if constexpr (DB > 0) {
-    const E* krb = p.kr + b0 * p.kr_sb + (int64_t)key * p.kr_ss;
-#pragma unroll
-    for (int kk = 0; kk < KB; ++kk) kf[KA + kk] = row8(krb + 16 * kk + 8 * h, key < nkeys);
-  }
-  const RowTile<E, DV, kBQ, 0> vt(w, lane);
+  for (int kk = 0; kk < KK; ++kk) kf[kk] = row8(kb + (int64_t)key * k_ss + 16 * kk + 8 * h, key < nkeys);
+  const RowTile<E, D, kBQ, 0> vt(w, lane);
   vt.issue(vimg, vb + (int64_t)k0 * v_ss, v_ss, nkeys - k0, w);
 
-  f32x16 dk[DTK], dv[DTV];  // dK^T, dV^T: [d][key]
+  f32x16 dk[DT], dv[DT];  // dK^T, dV^T: [d][key]
 #pragma unroll
-  for (int dt = 0; dt < DTK; ++dt) dk[dt] = (f32x16)(0.f);
-#pragma unroll
-  for (int dt = 0; dt < DTV; ++dt) dv[dt] = (f32x16)(0.f);
+  for (int dt = 0; dt < DT; ++dt) dk[dt] = (f32x16)(0.f), dv[dt] = (f32x16)(0.f);
 
-  RowFrag<DA, 1> qf(r, h);
-  RowFrag<DBX, 1> qrf(r, h);
-  RowFrag<DV, 1> df(r, h);
-  RowFrag<DV, 0> vf(r, h);
-  TrFrag<DA, 1> qt(h, i16, g4);
-  TrFrag<DBX, 1> qrt(h, i16, g4);
-  TrFrag<DV, 1> dt_(h, i16, g4);
-  const RowTile<E, DA, kBQ2, 1> qa(w, lane);
-  const RowTile<E, DBX, kBQ2, 1> qr(w, lane);
-  const RowTile<E, DV, kBQ2, 1> da(w, lane);
+  const RowFrag<D, 1> qf(r, h);
+  const RowFrag<D, 0> vf(r, h);
+  const TrFrag<D, 1> qt(h, i16, g4);
+  const RowTile<E, D, kBQP, 1> qd(w, lane);  // of Q and of dO
   const int64_t nrow = (int64_t)p.B * p.Hq * p.S;
   // the walk: sequence, head of the pair, 32-query tile (from the diagonal on under the causal mask)
-  const int t0 = causal ? k0 / kBQ2 : 0;
+  const int t0 = causal ? k0 / kBQP : 0;
   struct Cursor {
     int b, hp, t, nt, len;
   };
@@ -421,17 +410,16 @@ __global__ __launch_bounds__(kThreads, DB ? 1 : 2) void shared_bwd_dkdv_kernel(S
       c.b = c.b < 0 ? b0 : c.b + 1;
       if (c.b >= b1) return false;
       c.len = p.len(c.b);
-      c.nt = (c.len + kBQ2 - 1) / kBQ2;
+      c.nt = (c.len + kBQP - 1) / kBQP;
     }
     return true;
   };
   auto stage = [&](int buf, const Cursor& c) {
-    const int q0 = c.t * kBQ2, hd = hq + c.hp;
+    const int q0 = c.t * kBQP, hd = hq + c.hp;
     const E* qb = p.q + c.b * p.q_sb + hd * p.q_sh + (int64_t)q0 * p.q_ss;
     E* img = smem + buf * SLOT;
-    qa.issue(img, qb, p.q_ss, c.len - q0, w);
-    if constexpr (DB > 0) qr.issue(img + TA, qb + DA, p.q_ss, c.len - q0, w);
-    da.issue(img + TA + TB, p.dout + c.b * p.do_sb + hd * p.do_sh + (int64_t)q0 * p.do_ss, p.do_ss, c.len - q0, w);
+    qd.issue(img, qb, p.q_ss, c.len - q0, w);
+    qd.issue(img + TA, p.dout + c.b * p.do_sb + hd * p.do_sh + (int64_t)q0 * p.do_ss, p.do_ss, c.len - q0, w);
     if (w == 0) {
       const int q = min(q0 + (lane & 31), p.S - 1);  // rows past the length hold 0, 0 (and are masked)
       glds4(p.rows + (lane < 32 ? nrow : 0) + ((int64_t)c.b * p.Hq + hd) * p.S + q, &rc[buf][0]);
@@ -443,10 +431,10 @@ __global__ __launch_bounds__(kThreads, DB ? 1 : 2) void shared_bwd_dkdv_kernel(S
     vm_drain();       // this tile's LDS-DMA has landed ...
     __syncthreads();  // ... for every wave, and the other buffer's readers are done
     if (more) stage(buf ^ 1, next);
-    const int q0 = c.t * kBQ2;
-    if (causal && q0 + kBQ2 - 1 < kw0) return;
+    const int q0 = c.t * kBQP;
+    if (causal && q0 + kBQP - 1 < kw0) return;
     const E* qi = smem + buf * SLOT;
-    const E* di = qi + TA + TB;
+    const E* di = qi + TA;
     f32x16 s, dp;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -454,13 +442,13 @@ __global__ __launch_bounds__(kThreads, DB ? 1 : 2) void shared_bwd_dkdv_kernel(S
       s[i] = rc[buf][qr_];  // S - lse/scale  ->  P = exp2(that * scale * log2e)
       dp[i] = rc[buf][32 + qr_];
     }
-    const E* vi = vimg + 32 * w * DV;
+    const E* vi = vimg + 32 * w * D;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
-      s = mfma32(lds_read_b128(kk < KA ? qi + qf(kk) : qi + TA + qrf(kk - KA)), kf[kk], s);
-      if (kk < KV) dp = mfma32(lds_read_b128(di + df(kk)), lds_read_b128(vi + vf(kk)), dp);
+      s = mfma32(lds_read_b128(qi + qf(kk)), kf[kk], s);
+      dp = mfma32(lds_read_b128(di + qf(kk)), lds_read_b128(vi + vf(kk)), dp);
     }
-    if (uniform((causal && q0 < kw0 + 31) || q0 + kBQ2 > c.len || kw0 + 32 > nkeys)) {
+    if (uniform((causal && q0 < kw0 + 31) || q0 + kBQP > c.len || kw0 + 32 > nkeys)) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int q = q0 + (i & 3) + 8 * (i >> 2) + 4 * h;
@@ -475,15 +463,13 @@ __global__ __launch_bounds__(kThreads, DB ? 1 : 2) void shared_bwd_dkdv_kernel(S
     }
     const vec8_t<E> pf[2] = {pack8<E>(s, 0), pack8<E>(s, 8)}, dsf[2] = {pack8<E>(dp, 0), pack8<E>(dp, 8)};
 #pragma unroll
-    for (int dt = 0; dt < DTK; ++dt)
+    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2) {
-        if (dt < DTV) dv[dt] = mfma32(dt_.read(di, dt, 16 * s2), pf[s2], dv[dt]);
-        const vec8_t<E> a = dt < DTA ? qt.read(qi, dt, 16 * s2) : qrt.read(qi + TA, dt - DTA, 16 * s2);
-        dk[dt] = mfma32(a, dsf[s2], dk[dt]);
+        dv[dt] = mfma32(qt.read(di, dt, 16 * s2), pf[s2], dv[dt]);
+        dk[dt] = mfma32(qt.read(qi, dt, 16 * s2), dsf[s2], dk[dt]);
       }
   };
-  static_assert(DTV <= DTK, "the value's columns ride along the key's");
   Cursor cur{-1, 0, 0, 0, 0};
   if (k0 < nkeys && seek(cur)) {
     stage(0, cur);
@@ -507,23 +493,196 @@ __global__ __launch_bounds__(kThreads, DB ? 1 : 2) void shared_bwd_dkdv_kernel(S
   const int rows = pre ? p.P : p.S;
   const int nparts = (group / HP) * (pre ? p.nsplit : 1);
   const int slot = (pre ? part * (group / HP) : 0) + hh / HP;
-  const int64_t base = ((int64_t)(pre ? grp : b0) * rows + key);
-  if constexpr (DB > 0) {  // latent attention: one head owns its k_nope and v rows, the rope part is summed over heads
-    store_rows_bf16<DTA>(p.dk + base * p.dk_ss + hk * p.dk_sh, *reinterpret_cast<f32x16(*)[DTA]>(dk), p.scale, h, key < rows);
-    store_rows_bf16<DTV>(p.dv + base * p.dv_ss + hk * p.dv_sh, dv, 1.f, h, key < rows);
-    if (key < rows)
-      store_rows_f32<DB / 32>(p.dkr_part + (((int64_t)hq * p.B + b0) * p.S + key) * DB, dk + DTA, p.scale, h);
-  } else if (nparts == 1) {
-    E* dkp = pre ? p.dpk : p.dk;
-    E* dvp = pre ? p.dpv : p.dv;
-    store_rows_bf16<DTK>(dkp + (base * p.Hkv + hk) * DA, dk, p.scale, h, key < rows);
-    store_rows_bf16<DTV>(dvp + (base * p.Hkv + hk) * DV, dv, 1.f, h, key < rows);
+  const int64_t base = (int64_t)(pre ? grp : b0) * rows + key;
+  if (nparts == 1) {
+    store_rows_bf16<DT>((pre ? p.dpk : p.dk) + (base * p.Hkv + hk) * D, dk, p.scale, h, key < rows);
+    store_rows_bf16<DT>((pre ? p.dpv : p.dv) + (base * p.Hkv + hk) * D, dv, 1.f, h, key < rows);
   } else if (key < rows) {
     const int64_t all = (int64_t)(pre ? p.B / p.n : p.B) * rows;  // rows of a part
-    float* dkp = (pre ? p.dpk_part : p.dk_part) + ((slot * all + base) * p.Hkv + hk) * DA;
-    float* dvp = (pre ? p.dpv_part : p.dv_part) + ((slot * all + base) * p.Hkv + hk) * DV;
-    store_rows_f32<DTK>(dkp, dk, p.scale, h);
-    store_rows_f32<DTV>(dvp, dv, 1.f, h);
+    const int64_t at = ((slot * all + base) * p.Hkv + hk) * D;
+    store_rows_f32<DT>((pre ? p.dpk_part : p.dk_part) + at, dk, p.scale, h);
+    store_rows_f32<DT>((pre ? p.dpv_part : p.dv_part) + at, dv, 1.f, h);
+  }
+}
+
+// ---- dK / dV of latent attention: one workgroup per (b, head, 128 keys).
+// K, V, dK and dV of 32 keys are 240 registers at head dims 192 / 128: too many for two waves a SIMD, and one alone hides
+// none of its latencies (2120 us at S 8192, 32 heads). So two waves share 32 keys, and every SIMD runs one of each kind:
+//   the first   S_i = Q K^T, P_i = exp, P_i to LDS (fp32)  |  dV += P_i^T dO_i
+//   the second  dK += dS_{i-1}^T Q_{i-1}, dP_i = dO_i V^T  |  dS_i = P_i (dP_i - delta)
+// with a barrier at | and one per tile of 64 queries: the exponentials of one run beside the products of the other.
+template <typename E, int DA, int DB, int DV>
+__global__ __launch_bounds__(kKvThreads, 2) void latent_bwd_dkdv_kernel(SharedArgs<E> p) {
+  constexpr int KA = DA / 16, KB = DB / 16, KK = KA + KB, KV = DV / 16;
+  constexpr int DTK = (DA + DB) / 32, DTA = DA / 32, DTV = DV / 32;
+  constexpr int TA = kBQ2 * DA, TB = kBQ2 * DB, TO = kBQ2 * DV, SLOT = TA + TB + TO;
+  __shared__ __attribute__((aligned(16))) E smem[3 * SLOT];
+  __shared__ __attribute__((aligned(16))) float rc[3][2 * kBQ2];  // [buf][-lse/scale of the rows | -delta]
+  __shared__ __attribute__((aligned(16))) float pbuf[4][2][1024];  // [32 keys][32 queries]: P in accumulator order
+
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 31, h = lane >> 5, i16 = lane & 15, g4 = lane >> 4;
+  const int nkt = (p.S + kBQ - 1) / kBQ;
+  const int work = xcd_remap(blockIdx.x, gridDim.x);  // blocks of one (b, head) share their Q / dO stream
+  const int k0 = work % nkt * kBQ, hd = work / nkt % p.Hq, b = work / nkt / p.Hq;  // ascending: most queries first
+  const int len = p.len(b);
+  const int kg = w & 3, kw0 = k0 + 32 * kg, key = kw0 + r;
+  const RowTile<E, DA, kBQ2, 1, 8> qa(w, lane);
+  const RowTile<E, DB, kBQ2, 1, 8> qr(w, lane);
+  const RowTile<E, DV, kBQ2, 1, 8> da(w, lane);
+  const int64_t nrow = (int64_t)p.B * p.Hq * p.S;
+  const int t0 = p.causal ? k0 / kBQ2 : 0, nt = k0 < len ? (len + kBQ2 - 1) / kBQ2 : 0;
+  const E* qb = p.q + b * p.q_sb + hd * p.q_sh;
+  const E* dob = p.dout + b * p.do_sb + hd * p.do_sh;
+  const float* rowb = p.rows + (w == 0 ? nrow : 0) + ((int64_t)b * p.Hq + hd) * p.S;
+  auto stage = [&](int buf, int t) {
+    const int q0 = t * kBQ2;
+    E* img = smem + buf * SLOT;
+    qa.issue(img, qb + (int64_t)q0 * p.q_ss, p.q_ss, len - q0, w);
+    qr.issue(img + TA, qb + (int64_t)q0 * p.q_ss + DA, p.q_ss, len - q0, w);
+    da.issue(img + TA + TB, dob + (int64_t)q0 * p.do_ss, p.do_ss, len - q0, w);
+    // the rows' terms (rows past the length hold 0, 0 and are masked)
+    if (w < 2) glds4(rowb + min(q0 + lane, p.S - 1), &rc[buf][w * kBQ2]);
+  };
+  // both kinds of wave take the same walk: at tile t, tiles t - 1 and t are in LDS while t + 1 arrives, three buffers.
+  // first(buffer of t, of t - 1, t, whether t and t - 1 have work for these keys), second(buffer of t, whether)
+  auto walk = [&](auto&& first, auto&& second) {
+    if (t0 < nt) stage(0, t0);
+    bool behind = false;
+    int buf = 0, last = 2;
+    for (int t = t0; t < nt; ++t) {
+      vm_drain();
+      __syncthreads();  // tile t has landed for every wave, and the buffer of tile t - 2 has no reader left
+      const int free = 3 - buf - last;
+      if (t + 1 < nt) stage(free, t + 1);
+      const bool active = uniform(!(p.causal && t * kBQ2 + kBQ2 - 1 < kw0));
+      first(buf, last, t, active, behind);
+      __syncthreads();  // P of tile t is in LDS
+      second(buf, active);
+      behind = active;
+      last = buf, buf = free;
+    }
+    first(buf, last, nt, false, behind);
+  };
+
+  // keys past the length get zeros
+  const int64_t base = (int64_t)b * p.S + key;
+  if (w < 4) {  // P and dV
+    vec8_t<E> kf[KK];  // B operand of S = Q K^T
+    const E* kb = p.k + b * p.k_sb + hd * p.k_sh + (int64_t)key * p.k_ss + 8 * h;
+    const E* krb = p.kr + b * p.kr_sb + (int64_t)key * p.kr_ss + 8 * h;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) kf[kk] = row8(kk < KA ? kb + 16 * kk : krb + 16 * (kk - KA), key < len);
+    f32x16 dv[DTV];  // dV^T: [d][key]
+#pragma unroll
+    for (int dt = 0; dt < DTV; ++dt) dv[dt] = (f32x16)(0.f);
+    const RowFrag<DA, 1> qf0(r, h);
+    const RowFrag<DB, 1> qrf0(r, h);
+    const TrFrag<DV, 1> dt0(h, i16, g4);
+    vec8_t<E> pf[2][2];
+    walk(
+        [&](int buf, int, int t, bool active, bool) {
+          if (!active) return;
+          const int q0 = t * kBQ2;
+          RowFrag<DA, 1> qf = qf0;
+          RowFrag<DB, 1> qrf = qrf0;
+          qf.at += buf * SLOT, qrf.at += buf * SLOT + TA;
+          f32x16 s[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) s[u][j] = rc[buf][32 * u + (j & 3) + 8 * (j >> 2) + 4 * h];  // S - lse/scale
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+              s[u] = mfma32(lds_read_b128(smem + (kk < KA ? 32 * u * DA + qf(kk) : 32 * u * DB + qrf(kk - KA))), kf[kk], s[u]);
+          if (uniform((p.causal && q0 < kw0 + 31) || q0 + kBQ2 > len || kw0 + 32 > len)) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                const int q = q0 + 32 * u + (j & 3) + 8 * (j >> 2) + 4 * h;
+                if (key >= len || q >= len || (p.causal && key > q)) s[u][j] = -INFINITY;
+              }
+          }
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            float* to = pbuf[kg][u] + 4 * lane;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) s[u][j] = fast_exp2(s[u][j] * p.scale_log2);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              *reinterpret_cast<f32x4*>(to + 256 * j) = (f32x4){s[u][4 * j], s[u][4 * j + 1], s[u][4 * j + 2], s[u][4 * j + 3]};
+            pf[u][0] = pack8<E>(s[u], 0), pf[u][1] = pack8<E>(s[u], 8);
+          }
+        },
+        [&](int buf, bool active) {
+          if (!active) return;
+          TrFrag<DV, 1> dt_ = dt0;
+          dt_.at += buf * SLOT + TA + TB;
+#pragma unroll
+          for (int dt = 0; dt < DTV; ++dt)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) dv[dt] = mfma32(dt_.template read<E>(smem, dt, 16 * x), pf[x >> 1][x & 1], dv[dt]);
+        });
+    store_rows_bf16<DTV>(p.dv + base * p.dv_ss + hd * p.dv_sh, dv, 1.f, h, key < p.S);
+  } else {  // dS and dK, one tile behind
+    vec8_t<E> vf[KV];  // B operand of dP = dO V^T
+    const E* vb = p.v + b * p.v_sb + hd * p.v_sh + (int64_t)key * p.v_ss + 8 * h;
+#pragma unroll
+    for (int kk = 0; kk < KV; ++kk) vf[kk] = row8(vb + 16 * kk, key < len);
+    f32x16 dk[DTK];  // dK^T: [d][key]
+#pragma unroll
+    for (int dt = 0; dt < DTK; ++dt) dk[dt] = (f32x16)(0.f);
+    const RowFrag<DV, 1> df0(r, h);
+    const TrFrag<DA, 1> qt0(h, i16, g4);
+    const TrFrag<DB, 1> qrt0(h, i16, g4);
+    vec8_t<E> dsf[2][2];
+    f32x16 dp[2];
+    walk(
+        [&](int buf, int last, int, bool active, bool behind) {
+          if (behind) {
+            TrFrag<DA, 1> qt = qt0;
+            TrFrag<DB, 1> qrt = qrt0;
+            qt.at += last * SLOT, qrt.at += last * SLOT + TA;
+#pragma unroll
+            for (int dt = 0; dt < DTK; ++dt)
+#pragma unroll
+              for (int x = 0; x < 4; ++x)
+                dk[dt] = mfma32(dt < DTA ? qt.template read<E>(smem, dt, 16 * x) : qrt.template read<E>(smem, dt - DTA, 16 * x),
+                                dsf[x >> 1][x & 1], dk[dt]);
+          }
+          if (active) {
+            RowFrag<DV, 1> df = df0;
+            df.at += buf * SLOT + TA + TB;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int j = 0; j < 16; ++j) dp[u][j] = rc[buf][kBQ2 + 32 * u + (j & 3) + 8 * (j >> 2) + 4 * h];  // dP - delta
+#pragma unroll
+            for (int kk = 0; kk < KV; ++kk)
+#pragma unroll
+              for (int u = 0; u < 2; ++u) dp[u] = mfma32(lds_read_b128(smem + 32 * u * DV + df(kk)), vf[kk], dp[u]);
+          }
+        },
+        [&](int, bool active) {
+          if (!active) return;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const float* from = pbuf[kg][u] + 4 * lane;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const f32x4 pv = *reinterpret_cast<const f32x4*>(from + 256 * j);
+#pragma unroll
+              for (int x = 0; x < 4; ++x) dp[u][4 * j + x] *= pv[x];
+            }
+            dsf[u][0] = pack8<E>(dp[u], 0), dsf[u][1] = pack8<E>(dp[u], 8);
+          }
+        });
+    // one head owns its k_nope rows, the rope part is summed over the heads
+    store_rows_bf16<DTA>(p.dk + base * p.dk_ss + hd * p.dk_sh, *reinterpret_cast<f32x16(*)[DTA]>(dk), p.scale, h, key < p.S);
+    if (key < p.S) store_rows_f32<DB / 32>(p.dkr_part + (((int64_t)hd * p.B + b) * p.S + key) * DB, dk + DTA, p.scale, h);
   }
 }
 
@@ -676,10 +835,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> dlgm_latent_attn_bwd(const at::Te
     p.dkr_part = dkr_part.data_ptr<float>();
     if (dn == 128) {
       shared_bwd_dq_kernel<E, 128, 64, 128, false><<<blocks, kThreads, 0, stream>>>(p);
-      shared_bwd_dkdv_kernel<E, 128, 64, 128, false, 1><<<blocks, kThreads, 0, stream>>>(p);
+      latent_bwd_dkdv_kernel<E, 128, 64, 128><<<blocks, kKvThreads, 0, stream>>>(p);
     } else {
       shared_bwd_dq_kernel<E, 64, 32, 64, false><<<blocks, kThreads, 0, stream>>>(p);
-      shared_bwd_dkdv_kernel<E, 64, 32, 64, false, 1><<<blocks, kThreads, 0, stream>>>(p);
+      latent_bwd_dkdv_kernel<E, 64, 32, 64><<<blocks, kKvThreads, 0, stream>>>(p);
     }
     SumArgs<E> a{};
     a.part[0] = p.dkr_part, a.out[0] = ptr<E>(dkr), a.n[0] = B * S * dr, a.parts[0] = H;
@@ -781,8 +940,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> dlgm_pref
     auto run = [&](auto dc) {
       constexpr int DD = decltype(dc)::value;
       shared_bwd_dq_kernel<E, DD, 0, DD, true><<<q_blocks, kThreads, 0, stream>>>(p);
-      if (hp == 2) shared_bwd_dkdv_kernel<E, DD, 0, DD, true, 2><<<k_blocks, kThreads, 0, stream>>>(p);
-      else shared_bwd_dkdv_kernel<E, DD, 0, DD, true, 1><<<k_blocks, kThreads, 0, stream>>>(p);
+      if (hp == 2) prefix_bwd_dkdv_kernel<E, DD, 2><<<k_blocks, kThreads, 0, stream>>>(p);
+      else prefix_bwd_dkdv_kernel<E, DD, 1><<<k_blocks, kThreads, 0, stream>>>(p);
     };
     if (D == 128) run(std::integral_constant<int, 128>{});
     else run(std::integral_constant<int, 64>{});
