@@ -75,22 +75,28 @@ __global__ __launch_bounds__(kThreads) void latent_absorb_kernel(LatentArgs<E> p
   }
 }
 
-// One workgroup per (sequence, 64 heads, part of its length): tiles of 64 cache rows by LDS-DMA, one ahead. Scores: wave
-// (u, hb) takes 32 rows x 32 heads over all r + dr columns, its q operand in registers. Outputs: each wave takes r / 4
-// latent columns of all 64 heads; the weights pass through LDS in fragment order. 64 heads a workgroup keep the cache rows'
-// LDS reads (36 KiB a wave and tile at r 512) below the matrix time (68 MFMA) with one wave a SIMD.
+// One workgroup per (sequence, 64 heads, part of its length): tiles of 64 cache rows by LDS-DMA, one ahead (two tiles fill a
+// CU's LDS, so its 8 waves are two a SIMD). Scores: the waves (u, hb, kd) take 32 rows x 32 heads over half of the r + dr
+// columns each, q in registers; the halves meet in LDS, where each of a pair keeps 16 of the 32 rows: their weights go back
+// to LDS as matrix operands. Outputs: each wave takes r / 8 latent columns of all 64 heads. 64 heads a workgroup keep LDS
+// reads (every wave reads 32 rows of half the columns: 147 KiB a tile, 64 KiB of it again transposed) beside the matrix
+// products (68 a SIMD). With 4 waves over whole rows, one a SIMD, 128 heads over 32 x 16384 tokens took 300 us.
+constexpr int kLatentThreads = 512;
+
 template <typename E, int R, int DR>
-__global__ __launch_bounds__(kThreads, 1) void latent_attend_kernel(LatentArgs<E> p) {
-  constexpr int NI = R / 128, KR = R / 16, KK = KR + DR / 16;  // images, k-steps
+__global__ __launch_bounds__(kLatentThreads, 2) void latent_attend_kernel(LatentArgs<E> p) {
+  constexpr int NI = R / 128, KR = R / 16, KK = KR + DR / 16, KH = KK / 2;  // images, k-steps, a wave's k-steps
   constexpr int TI = 64 * 128, SLOT = 64 * (R + DR);
-  constexpr int DT = R / 128;  // 32-column output tiles of a wave
+  constexpr int DT = R / 256;  // 32-column output tiles of a wave
+  static_assert(KK % 2 == 0, "the columns split evenly over a pair of waves");
   __shared__ __attribute__((aligned(16))) E smem[2 * SLOT];
-  __shared__ __attribute__((aligned(16))) E pbuf[8 * 512];  // [u][s2][hb] fragments of 64 lanes x 8
-  __shared__ float smax[2][64], ssum[2][64];
+  // 2 KiB a wave: its partner's half of the scores (2 KiB); then, written by the partner, who alone has read them: a
+  // fragment of weights (1 KiB), the maxima of 32 heads and whether one outgrew the reference
+  __shared__ __attribute__((aligned(16))) float xbuf[8][512];
 
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 31, h = lane >> 5, i16 = lane & 15, g4 = lane >> 4;
-  const int u = w & 1, hb = w >> 1;
+  const int u = w & 1, hb = (w >> 1) & 1;
   const int nhb = (p.H + 63) / 64;
   // head blocks of one (sequence, part) read the same rows: they follow each other on one XCD
   const int work = xcd_remap(blockIdx.x, gridDim.x);
@@ -98,17 +104,10 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attend_kernel(LatentArgs<E
   const int len = p.len(b);
   const int tiles = (len + 63) / 64;
   const int t0 = (int)((int64_t)tiles * part / p.ns), t1 = (int)((int64_t)tiles * (part + 1) / p.ns);
+  const int blocks = head0 + 32 < p.H ? 2 : 1;  // of 32 heads that exist
 
-  const int head = head0 + 32 * hb + r;
-  vec8_t<E> qf[KK];
-  {
-    const E* qa = p.qa + ((int64_t)b * p.H + head) * R + 8 * h;
-    const E* qr = p.q + b * p.q_sb + head * p.q_sh + p.dn + 8 * h;
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) qf[kk] = row8(kk < KR ? qa + 16 * kk : qr + 16 * (kk - KR), head < p.H);
-  }
-  const RowTile<E, 128, 64, 1> ct(w, lane);
-  const RowTile<E, DR, 64, 0> rt(w, lane);
+  const RowTile<E, 128, 64, 1, 8> ct(w, lane);
+  const RowTile<E, DR, 64, 0, 8> rt(w, lane);
   const E* cb = p.cache + b * p.c_sb;
   auto stage = [&](int buf, int t) {
     E* img = smem + buf * SLOT;
@@ -123,86 +122,131 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attend_kernel(LatentArgs<E
   for (int x = 0; x < 2; ++x)
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[x][dt] = (f32x16)(0.f);
-  RowFrag<128, 1> cf(r, h);
-  RowFrag<DR, 0> rf(r, h);
-  TrFrag<128, 1> vf(h, i16, g4);
-  float m_run[2] = {-INFINITY, -INFINITY}, l_run = 0.f;  // maxima of heads r and 32 + r; the sum of this wave's rows
+  float m_run[2] = {-INFINITY, -INFINITY}, l_run = 0.f;  // reference of heads r and 32 + r; the sum over this wave's rows
 
-  auto tile = [&](auto bufc, int t) {
-    constexpr int buf = decltype(bufc)::value;
-    vm_drain();
-    __syncthreads();
-    if (t + 1 < t1) stage(buf ^ 1, t + 1);
-    const E* img = smem + buf * SLOT;
-    pin(cf.at), pin(rf.at), pin(vf.at);
-    f32x16 s = (f32x16)(0.f);
+  auto walk = [&](auto kdc) {
+    constexpr int KD = decltype(kdc)::value;
+    const int head = head0 + 32 * hb + r;
+    vec8_t<E> qf[KH];
+    {
+      const E* qa = p.qa + ((int64_t)b * p.H + head) * R + 8 * h;
+      const E* qr = p.q + b * p.q_sb + head * p.q_sh + p.dn + 8 * h;
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      const E* a = kk < KR ? img + kk / 8 * TI + 32 * u * 128 + cf(kk % 8) : img + NI * TI + 32 * u * DR + rf(kk - KR);
-      s = mfma32(lds_read_b128(a), qf[kk], s);
-    }
-    if (uniform(t * 64 + 64 > len)) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (t * 64 + 32 * u + (i & 3) + 8 * (i >> 2) + 4 * h >= len) s[i] = -INFINITY;
-    }
-    float mx = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[i]);
-    mx = fmaxf(mx, swap_halves(mx)) * p.scale_log2;
-    if (h == 0) smax[u][32 * hb + r] = mx;
-    __syncthreads();
-    // every wave follows the maxima of all 64 heads, so the weights of a tile share one reference
-    float mt[2];
-#pragma unroll
-    for (int x = 0; x < 2; ++x) mt[x] = fmaxf(smax[0][32 * x + r], smax[1][32 * x + r]);
-    if (__any(mt[0] > m_run[0] + kRescaleLog2 || mt[1] > m_run[1] + kRescaleLog2)) {
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const float m_new = fmaxf(m_run[x], mt[x]);
-        const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run[x] - m_new);
-        m_run[x] = m_new;
-        if (x == hb) l_run *= alpha;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[x][dt] *= alpha;
+      for (int j = 0; j < KH; ++j) {
+        const int kk = KD * KH + j;
+        qf[j] = row8(kk < KR ? qa + 16 * kk : qr + 16 * (kk - KR), head < p.H);
       }
     }
-    const float m_own = hb ? m_run[1] : m_run[0];
-    const float m_use = m_own == -INFINITY ? 0.f : m_own;
+    RowFrag<128, 1> cf0(r, h);
+    RowFrag<DR, 0> rf0(r, h);
+    TrFrag<128, 1> vf0(h, i16, g4);
+    float* const mine = xbuf[2 * (2 * KD + hb) + u];
+    float* const theirs = xbuf[2 * (2 * (1 - KD) + hb) + u];
+    if (t0 < t1) stage(0, t0);
+    for (int t = t0, buf = 0; t < t1; ++t, buf ^= 1) {
+      vm_drain();
+      __syncthreads();
+      if (t + 1 < t1) stage(buf ^ 1, t + 1);
+      const E* img = smem + buf * SLOT;
+      f32x16 s = (f32x16)(0.f);
+      if (hb < blocks) {
+        RowFrag<128, 1> cf = cf0;
+        RowFrag<DR, 0> rf = rf0;
+        cf.at += 32 * u * 128, rf.at += NI * TI + 32 * u * DR;
+        pin(cf.at), pin(rf.at);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s[i] = fast_exp2(s[i] * p.scale_log2 - m_use);
-      l_run += s[i];
-    }
+        for (int j = 0; j < KH; ++j) {
+          const int kk = KD * KH + j;
+          s = mfma32(lds_read_b128(img + (kk < KR ? kk / 8 * TI + cf(kk % 8) : rf(kk - KR))), qf[j], s);
+        }
+      }
+      // each of the pair keeps the 16 rows whose scores are registers 8 KD .. 8 KD + 7
 #pragma unroll
-    for (int s2 = 0; s2 < 2; ++s2)
-      *reinterpret_cast<vec8_t<E>*>(pbuf + ((2 * u + s2) * 2 + hb) * 512 + lane * 8) = pack8<E>(s, 8 * s2);
-    __syncthreads();
-    vec8_t<E> pf[2][4];
+      for (int j = 0; j < 2; ++j)
+        *reinterpret_cast<f32x4*>(mine + 256 * j + 4 * lane) =
+            (f32x4){s[8 - 8 * KD + 4 * j], s[8 - 8 * KD + 4 * j + 1], s[8 - 8 * KD + 4 * j + 2], s[8 - 8 * KD + 4 * j + 3]};
+      __syncthreads();
+      float v[8];
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
+      for (int j = 0; j < 2; ++j) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(theirs + 256 * j + 4 * lane);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) pf[x][k] = lds_read_b128(pbuf + (2 * k + x) * 512 + lane * 8);
+        for (int i = 0; i < 4; ++i) v[4 * j + i] = s[8 * KD + 4 * j + i] + x[i];
+      }
+      if (uniform(t * 64 + 64 > len)) {
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      const int col = w * DT + dt;  // 32-column tile of the latent vector
-      const E* vi = img + col / 4 * TI;
+        for (int j = 0; j < 8; ++j)
+          if (t * 64 + 32 * u + 16 * KD + (j & 3) + 8 * (j >> 2) + 4 * h >= len) v[j] = -INFINITY;
+      }
+      float mx = v[0];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const vec8_t<E> a = vf.read(vi, col % 4, 16 * k);
-        o[0][dt] = mfma32(a, pf[0][k], o[0][dt]);
-        o[1][dt] = mfma32(a, pf[1][k], o[1][dt]);
+      for (int j = 1; j < 8; ++j) mx = fmaxf(mx, v[j]);
+      mx = fmaxf(mx, swap_halves(mx)) * p.scale_log2;
+      const float m_own = hb ? m_run[1] : m_run[0];
+      const bool grown = __any(mx > m_own + kRescaleLog2);
+      // weights over the reference so far: right unless a head outgrew it by 2^kRescaleLog2, which is seen at the barrier
+      auto weigh = [&](float m) {
+        const float m_use = m == -INFINITY ? 0.f : m;
+        float e[8], sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          e[j] = fast_exp2(v[j] * p.scale_log2 - m_use);
+          sum += e[j];
+        }
+        *reinterpret_cast<vec8_t<E>*>(theirs + 4 * lane) =
+            (vec8_t<E>){(E)e[0], (E)e[1], (E)e[2], (E)e[3], (E)e[4], (E)e[5], (E)e[6], (E)e[7]};
+        return sum;
+      };
+      float sum = weigh(m_own);
+      if (h == 0) theirs[256 + r] = mx;
+      if (lane == 0) theirs[288] = grown ? 1.f : 0.f;
+      __syncthreads();
+      if (__any(xbuf[lane & 7][288] != 0.f)) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float m_new = m_run[x];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) m_new = fmaxf(m_new, xbuf[4 * (k >> 1) + 2 * x + (k & 1)][256 + r]);
+          const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run[x] - m_new);
+          m_run[x] = m_new;
+          if (x == hb) l_run *= alpha;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) o[x][dt] *= alpha;
+        }
+        sum = weigh(hb ? m_run[1] : m_run[0]);
+        __syncthreads();
+      }
+      l_run += sum;
+      // weights of 64 rows: fragment (u, s2, head block x) lies with wave (u, x, 1 - s2)
+      vec8_t<E> pf[2][4];
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          pf[x][k] = *reinterpret_cast<const vec8_t<E>*>(xbuf[2 * (2 * (1 - (k & 1)) + x) + (k >> 1)] + 4 * lane);
+      TrFrag<128, 1> vf = vf0;
+      pin(vf.at);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const int col = w * DT + dt;  // 32-column tile of the latent vector
+        TrFrag<128, 1> vc = vf;
+        vc.at ^= (col % 4) << 5;
+        const E* vi = img + col / 4 * TI;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const vec8_t<E> a = vc.read(vi, 0, 16 * k);
+          o[0][dt] = mfma32(a, pf[0][k], o[0][dt]);
+          if (blocks > 1) o[1][dt] = mfma32(a, pf[1][k], o[1][dt]);
+        }
       }
     }
   };
-  if (t0 < t1) stage(0, t0);
-  for (int t = t0; t < t1; t += 2) {
-    tile(std::integral_constant<int, 0>{}, t);
-    if (t + 1 < t1) tile(std::integral_constant<int, 1>{}, t + 1);
-  }
+  if (w < 4) walk(std::integral_constant<int, 0>{});
+  else walk(std::integral_constant<int, 1>{});
 
-  const float l_half = l_run + swap_halves(l_run);
-  if (h == 0) ssum[u][32 * hb + r] = l_half;
+  const float l_pair = l_run + swap_halves(l_run);
+  __syncthreads();  // the last tile's weights have been read
+  if (h == 0) xbuf[w][r] = l_pair;
   __syncthreads();
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
@@ -211,50 +255,60 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attend_kernel(LatentArgs<E
     const int64_t slot = ((int64_t)b * p.H + hd) * p.ns + part;
     if (w == 0 && h == 0) {
       p.ml[2 * slot] = m_run[x];
-      p.ml[2 * slot + 1] = ssum[0][32 * x + r] + ssum[1][32 * x + r];
+      p.ml[2 * slot + 1] = (xbuf[2 * x][r] + xbuf[2 * x + 1][r]) + (xbuf[4 + 2 * x][r] + xbuf[4 + 2 * x + 1][r]);
     }
     if (t0 < t1) store_rows_f32<DT>(p.o + slot * R + w * DT * 32, o[x], 1.f, h);  // an empty part is not read
   }
 }
 
-// One workgroup per (head, 32 sequences): join the parts into the latent output (16 bits in LDS, the operand of the
-// product), then out = W_v[h] o.
+// One workgroup per (head, 8 sequences): a wave joins the parts of two of them into the latent output, then out = W_v[h] o.
+// The latent output enters its product as two 16-bit terms (value and remainder), so it is not rounded: the product is a
+// small part of the call.
+constexpr int kProjectRows = 8;
 template <typename E, int R, int DV>
 __global__ __launch_bounds__(kThreads) void latent_project_kernel(LatentArgs<E> p) {
   constexpr int LD = R + 8;
-  __shared__ __attribute__((aligned(16))) E ol[32 * LD];
+  __shared__ __attribute__((aligned(16))) E ol[2][kProjectRows * LD];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 31, h = lane >> 5;
-  const int head = blockIdx.x % p.H, b0 = blockIdx.x / p.H * 32;
-  const int col = lane * 8;
-  for (int k = w; k < 32; k += 4) {
+  const int work = xcd_remap(blockIdx.x, gridDim.x), nb = (p.B + kProjectRows - 1) / kProjectRows;
+  const int head = work / nb, b0 = work % nb * kProjectRows;  // workgroups of one head read the same W_v
+  const int col = lane * 8 % R;  // r 256: the upper lanes repeat the lower (readlane below needs all of them to run)
+  for (int k = w; k < kProjectRows; k += 4) {
     const int b = b0 + k;
     f32x8 acc = (f32x8)(0.f);
-    float l = 0.f;
     if (b < p.B) {
       const int64_t slot = ((int64_t)b * p.H + head) * p.ns;
-      float m = -INFINITY;
-      for (int s = 0; s < p.ns; ++s) m = fmaxf(m, p.ml[2 * (slot + s)]);
+      float ms = -INFINITY, ls = 0.f;  // of part `lane` (at most 64 parts)
+      if (lane < p.ns) ms = p.ml[2 * (slot + lane)], ls = p.ml[2 * (slot + lane) + 1];
+      const float m = wave_max(ms);
+      float f = ls == 0.f ? 0.f : fast_exp2(ms - m);  // an empty part (a NaN sum is none)
+      const float l = wave_sum(f * ls);
+      f = l == 0.f ? 0.f : f / l;  // a sequence without keys: zeros
+#pragma unroll 4
       for (int s = 0; s < p.ns; ++s) {
-        const float ls = p.ml[2 * (slot + s) + 1];
-        if (ls == 0.f) continue;  // an empty part (a NaN sum is none)
-        const float f = fast_exp2(p.ml[2 * (slot + s)] - m);
-        l += f * ls;
-        if (col < R) acc += load8(p.o + (slot + s) * R + col) * f;
+        const float fs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s));
+        if (fs == 0.f) continue;  // nothing was written there
+        acc += load8(p.o + (slot + s) * R + col) * fs;
       }
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;  // a sequence without keys: zeros
-    if (col < R) store8f(ol + k * LD + col, acc * inv);
+    const vec8_t<E> hi = __builtin_convertvector(acc, vec8_t<E>);
+    *reinterpret_cast<vec8_t<E>*>(ol[0] + k * LD + col) = hi;
+    store8f(ol[1] + k * LD + col, acc - __builtin_convertvector(hi, f32x8));
   }
   __syncthreads();
   if (w >= DV / 32) return;
   const E* wv = p.w + ((int64_t)head * (p.dn + p.dv) + p.dn + 32 * w + r) * p.w_ss + 8 * h;
+  const int at = r % kProjectRows * LD + 8 * h;  // columns past the sequences repeat them and are not stored
   f32x16 acc = (f32x16)(0.f);
-#pragma unroll 8
-  for (int kk = 0; kk < R / 16; ++kk)
-    acc = mfma32(*reinterpret_cast<const vec8_t<E>*>(wv + 16 * kk), lds_read_b128(ol + r * LD + 16 * kk + 8 * h), acc);
+#pragma unroll 16
+  for (int kk = 0; kk < R / 16; ++kk) {
+    const vec8_t<E> a = *reinterpret_cast<const vec8_t<E>*>(wv + 16 * kk);
+    acc = mfma32(a, lds_read_b128(ol[0] + at + 16 * kk), acc);
+    acc = mfma32(a, lds_read_b128(ol[1] + at + 16 * kk), acc);
+  }
   const f32x16 acc1[1] = {acc};
-  store_rows_bf16<1>(p.out + ((int64_t)(b0 + r) * p.H + head) * DV + 32 * w, acc1, 1.f, h, b0 + r < p.B);
+  store_rows_bf16<1>(p.out + ((int64_t)(b0 + r) * p.H + head) * DV + 32 * w, acc1, 1.f, h, r < kProjectRows && b0 + r < p.B);
 }
 
 // ---- shared prefix ------------------------------------------------------------------------------
@@ -275,18 +329,18 @@ struct PrefixArgs {
   float scale_log2;
 };
 
-// One workgroup per (kv head, block of rows, part of a key range): 128 keys a step by LDS-DMA, one step ahead. The rows
-// are (sequence of the group, q head of the kv head) for the prefix and the q heads for a sequence's own keys. rw of the 4
-// waves stand along the rows, so few rows leave the waves to share the 128 keys (joined through LDS at the end) and many
-// rows read each key once for 128 of them.
+// One workgroup per (kv head, block of rows, part of a key range): 64 keys a step by LDS-DMA, one step ahead, two workgroups
+// a CU. The rows are (sequence of the group, q head of the kv head) for the prefix and the q heads for a sequence's own
+// keys. rw of the 4 waves stand along the rows: 128 rows take a step's keys whole, 64 share its two halves between pairs of
+// waves, 32 between two waves -- few rows are bound by the cache alone, which all 4 waves load.
+constexpr int kStep = 64;
 template <typename E, int D>
-__global__ __launch_bounds__(kThreads, 1) void prefix_attend_kernel(PrefixArgs<E> p) {
-  constexpr int KK = D / 16, DT = D / 32, KEYS = 128;
-  constexpr int TI = KEYS * D, SLOT = 2 * TI;
-  constexpr int LDO = D + 4;
+__global__ __launch_bounds__(kThreads, 2) void prefix_attend_kernel(PrefixArgs<E> p) {
+  constexpr int KK = D / 16, DT = D / 32;
+  constexpr int TI = kStep * D, SLOT = 2 * TI;
   __shared__ __attribute__((aligned(16))) E smem[2 * SLOT];
   __shared__ float sm[4][32], sl[4][32];
-  static_assert(sizeof(E) * 2 * SLOT >= 4 * 32 * LDO * 4, "the joined rows fit the tiles' space");
+  static_assert(sizeof(E) * 2 * SLOT == 4 * 32 * D * 4, "the rows of four waves fit the tiles' space");
 
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 31, h = lane >> 5, i16 = lane & 15, g4 = lane >> 4;
@@ -318,21 +372,21 @@ __global__ __launch_bounds__(kThreads, 1) void prefix_attend_kernel(PrefixArgs<E
     kb = p.k + b0 * p.k_sb + hk * p.k_sh, vb = p.v + b0 * p.v_sb + hk * p.v_sh;
     k_ss = p.k_ss, v_ss = p.v_ss;
   }
-  const int kw = w / rw;  // this wave's share of a step's keys: rw blocks of 32 from block kw rw on
+  const int kw = w / rw;  // which half of a step's keys, where the rows leave waves to share them (others: none)
   const int idx = (rb * rw + w % rw) * 32 + r, seq = b0 + idx / rep, hq = hk * rep + idx % rep;
   const bool ok = idx < nrows;
-  const int steps = (len + KEYS - 1) / KEYS;
+  const int steps = (len + kStep - 1) / kStep;
   const int t0 = (int)((int64_t)steps * part / nparts), t1 = (int)((int64_t)steps * (part + 1) / nparts);
 
   vec8_t<E> qf[KK];
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) qf[kk] = row8(p.q + seq * p.q_sb + hq * p.q_sh + 16 * kk + 8 * h, ok);
-  const RowTile<E, D, KEYS, 0> kt(w, lane);
-  const RowTile<E, D, KEYS, 2> vt(w, lane);
+  const RowTile<E, D, kStep, 0> kt(w, lane);
+  const RowTile<E, D, kStep, 2> vt(w, lane);
   auto stage = [&](int buf, int t) {
     E* img = smem + buf * SLOT;
-    kt.issue(img, kb + (int64_t)t * KEYS * k_ss, k_ss, len - t * KEYS, w);
-    vt.issue(img + TI, vb + (int64_t)t * KEYS * v_ss, v_ss, len - t * KEYS, w);
+    kt.issue(img, kb + (int64_t)t * kStep * k_ss, k_ss, len - t * kStep, w);
+    vt.issue(img + TI, vb + (int64_t)t * kStep * v_ss, v_ss, len - t * kStep, w);
   };
   f32x16 o[DT];
 #pragma unroll
@@ -340,56 +394,73 @@ __global__ __launch_bounds__(kThreads, 1) void prefix_attend_kernel(PrefixArgs<E
   float m_run = -INFINITY, l_run = 0.f;
   const RowFrag<D, 0> kf(r, h);
   const TrFrag<D, 2> vf(h, i16, g4);
+  // U blocks of 32 keys from block blk on
+  auto blocks = [&](auto uc, const E* ki, int key0) {
+    constexpr int U = decltype(uc)::value;
+    const E* vi = ki + TI;
+    f32x16 s[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) s[u] = (f32x16)(0.f);
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+      for (int u = 0; u < U; ++u) s[u] = mfma32(lds_read_b128(ki + 32 * u * D + kf(kk)), qf[kk], s[u]);
+    if (uniform(key0 + 32 * U > len)) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (key0 + 32 * u + (i & 3) + 8 * (i >> 2) + 4 * h >= len) s[u][i] = -INFINITY;
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[u][i]);
+    mx = fmaxf(mx, swap_halves(mx)) * p.scale_log2;
+    if (__any(mx > m_run + kRescaleLog2)) {
+      const float m_new = fmaxf(m_run, mx);
+      const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
+    }
+    const float m_use = m_run == -INFINITY ? 0.f : m_run;
+    vec8_t<E> pf[U][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[u][i] = fast_exp2(s[u][i] * p.scale_log2 - m_use);
+        l_run += s[u][i];
+      }
+      pf[u][0] = pack8<E>(s[u], 0), pf[u][1] = pack8<E>(s[u], 8);
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2) o[dt] = mfma32(vf.read(vi, dt, 32 * u + 16 * s2), pf[u][s2], o[dt]);
+  };
   if (t0 < t1) stage(0, t0);
   for (int t = t0; t < t1; ++t) {
     vm_drain();
     __syncthreads();
     const int buf = (t - t0) & 1;
     if (t + 1 < t1) stage(buf ^ 1, t + 1);
-    for (int x = 0; x < rw; ++x) {
-      const int blk = kw * rw + x, key0 = t * KEYS + 32 * blk;
-      if (key0 >= len) break;
-      const E* ki = smem + buf * SLOT + blk * 32 * D;
-      const E* vi = ki + TI;
-      f32x16 s = (f32x16)(0.f);
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) s = mfma32(lds_read_b128(ki + kf(kk)), qf[kk], s);
-      if (uniform(key0 + 32 > len)) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (key0 + (i & 3) + 8 * (i >> 2) + 4 * h >= len) s[i] = -INFINITY;
-      }
-      float mx = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[i]);
-      mx = fmaxf(mx, swap_halves(mx)) * p.scale_log2;
-      if (__any(mx > m_run + kRescaleLog2)) {
-        const float m_new = fmaxf(m_run, mx);
-        const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
-        m_run = m_new;
-        l_run *= alpha;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
-      }
-      const float m_use = m_run == -INFINITY ? 0.f : m_run;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[i] = fast_exp2(s[i] * p.scale_log2 - m_use);
-        l_run += s[i];
-      }
-      const vec8_t<E> pf[2] = {pack8<E>(s, 0), pack8<E>(s, 8)};
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int s2 = 0; s2 < 2; ++s2) o[dt] = mfma32(vf.read(vi, dt, 16 * s2), pf[s2], o[dt]);
-    }
+    const E* ki = smem + buf * SLOT;
+    const int key0 = t * kStep + 32 * kw;
+    if (rw == 4) blocks(std::integral_constant<int, 2>{}, ki, key0);
+    else if (kw < 2 && key0 < len) blocks(std::integral_constant<int, 1>{}, ki + 32 * kw * D, key0);
   }
 
   const int slots = p.np + p.no, slot = pre ? part : p.np + part;
-  const int64_t at = ((int64_t)seq * p.Hq + hq) * slots + slot;
-  float l = l_run + swap_halves(l_run);
+  const float l = l_run + swap_halves(l_run);
   if (rw == 4) {  // no other wave has these rows
     if (ok) {
+      const int64_t at = ((int64_t)seq * p.Hq + hq) * slots + slot;
       if (h == 0) p.ml[2 * at] = m_run, p.ml[2 * at + 1] = l;
       if (t0 < t1) store_rows_f32<DT>(p.o + at * D, o, 1.f, h);  // an empty part is not read
     }
@@ -397,27 +468,34 @@ __global__ __launch_bounds__(kThreads, 1) void prefix_attend_kernel(PrefixArgs<E
   }
   if (h == 0) sm[w][r] = m_run, sl[w][r] = l;
   __syncthreads();  // also: the last tiles have been read
-  float m = -INFINITY;
-  for (int x = w % rw; x < 4; x += rw) m = fmaxf(m, sm[x][r]);
+  const float m = fmaxf(sm[w % rw][r], sm[w % rw + rw][r]);
   const float f = l == 0.f ? 0.f : fast_exp2(m_run - m);
-  float* joined = reinterpret_cast<float*>(smem);
-  store_rows_f32<DT>(joined + (w * 32 + r) * LDO, o, f, h);
+  float* joined = reinterpret_cast<float*>(smem);  // rows of D floats, each turned by 4 per row so that no bank repeats
+  if (kw < 2) {
+    float* row = joined + (w * 32 + r) * D;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 v = {o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
+        *reinterpret_cast<f32x4*>(row + ((dt * 32 + 8 * g + 4 * h + 4 * r) & (D - 1))) = v * f;
+      }
+  }
   __syncthreads();
-  // the rw blocks of 32 rows, summed over the 4 / rw waves that shared their keys
   for (int i = threadIdx.x; i < rw * 32 * (D / 4); i += kThreads) {
-    const int row = i / (D / 4), c = i % (D / 4) * 4, x0 = row >> 5, rr = row & 31;
-    const int id = (rb * rw + x0) * 32 + rr;
+    const int row = i / (D / 4), c = i % (D / 4) * 4, x = row >> 5, rr = row & 31;
+    const int id = (rb * rw + x) * 32 + rr;
     if (id >= nrows) break;
-    float mm = -INFINITY, ll = 0.f;
-    f32x4 acc = (f32x4)(0.f);
-    for (int x = x0; x < 4; x += rw) mm = fmaxf(mm, sm[x][rr]);
-    for (int x = x0; x < 4; x += rw) {
-      ll += sl[x][rr] == 0.f ? 0.f : sl[x][rr] * fast_exp2(sm[x][rr] - mm);
-      acc += *reinterpret_cast<const f32x4*>(joined + (x * 32 + rr) * LDO + c);
-    }
     const int64_t a = ((int64_t)(b0 + id / rep) * p.Hq + hk * rep + id % rep) * slots + slot;
-    if (c == 0) p.ml[2 * a] = mm, p.ml[2 * a + 1] = ll;
-    if (t0 < t1) *reinterpret_cast<f32x4*>(p.o + a * D + c) = acc;
+    const int turned = (c + 4 * rr) & (D - 1);
+    if (c == 0) {
+      const float m0 = sm[x][rr], m1 = sm[x + rw][rr], l0 = sl[x][rr], l1 = sl[x + rw][rr], mm = fmaxf(m0, m1);
+      p.ml[2 * a] = mm;
+      p.ml[2 * a + 1] = (l0 == 0.f ? 0.f : l0 * fast_exp2(m0 - mm)) + (l1 == 0.f ? 0.f : l1 * fast_exp2(m1 - mm));
+    }
+    if (t0 < t1)
+      *reinterpret_cast<f32x4*>(p.o + a * D + c) = *reinterpret_cast<const f32x4*>(joined + row * D + turned) +
+                                                    *reinterpret_cast<const f32x4*>(joined + (row + rw * 32) * D + turned);
   }
 }
 
@@ -425,29 +503,35 @@ __global__ __launch_bounds__(kThreads, 1) void prefix_attend_kernel(PrefixArgs<E
 template <typename E, int D>
 __global__ __launch_bounds__(kThreads) void prefix_join_kernel(PrefixArgs<E> p) {
   constexpr int V = D / 64;  // columns of a lane
-  __shared__ float red[4][D], sl[4];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int slots = p.np + p.no;
+  __shared__ float red[4][D];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int slots = p.np + p.no;  // at most 128
   const int64_t row = blockIdx.x, base = row * slots;
-  float m = -INFINITY, l = 0.f, acc[V] = {};
-  for (int s = 0; s < slots; ++s) m = fmaxf(m, p.ml[2 * (base + s)]);
-  for (int s = w; s < slots; s += 4) {
-    const float ls = p.ml[2 * (base + s) + 1];
-    if (ls == 0.f) continue;  // an empty part (a NaN sum is none)
-    const float f = fast_exp2(p.ml[2 * (base + s)] - m);
-    l += f * ls;
+  float ms[2] = {-INFINITY, -INFINITY}, ls[2] = {0.f, 0.f}, l = 0.f, acc[V] = {};
 #pragma unroll
-    for (int j = 0; j < V; ++j) acc[j] += f * p.o[(base + s) * D + lane * V + j];
+  for (int x = 0; x < 2; ++x)
+    if (64 * x + lane < slots) ms[x] = p.ml[2 * (base + 64 * x + lane)], ls[x] = p.ml[2 * (base + 64 * x + lane) + 1];
+  const float m = wave_max(fmaxf(ms[0], ms[1]));
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const float f = ls[x] == 0.f ? 0.f : fast_exp2(ms[x] - m);  // an empty part (a NaN sum is none)
+    l += f * ls[x];
+#pragma unroll 4
+    for (int s = 64 * x + w; s < min(slots, 64 * x + 64); s += 4) {
+      const float fs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s & 63));
+      if (fs == 0.f) continue;  // nothing was written there
+#pragma unroll
+      for (int j = 0; j < V; ++j) acc[j] += fs * p.o[(base + s) * D + lane * V + j];
+    }
   }
+  l = wave_sum(l);
 #pragma unroll
   for (int j = 0; j < V; ++j) red[w][lane * V + j] = acc[j];
-  if (lane == 0) sl[w] = l;
   __syncthreads();
   if (threadIdx.x >= D) return;
   const int c = threadIdx.x;
-  const float lt = sl[0] + sl[1] + sl[2] + sl[3];
   const float o = red[0][c] + red[1][c] + red[2][c] + red[3][c];
-  p.out[row * D + c] = (E)(lt == 0.f ? 0.f : o / lt);  // a row without keys: zeros
+  p.out[row * D + c] = (E)(l == 0.f ? 0.f : o / l);  // a row without keys: zeros
 }
 
 // how many parts a length of `steps` steps is cut into so that `items` such lengths give about `want` workgroups
@@ -488,8 +572,8 @@ at::Tensor dlgm_latent_attn_decode(const at::Tensor& q, const at::Tensor& cache,
   auto qa = at::empty({B, H, r}, q.options());
   auto o = at::empty({B, H, ns, r}, q.options().dtype(at::kFloat));
   auto ml = at::empty({B, H, ns, 2}, q.options().dtype(at::kFloat));
-  const int64_t a_blocks = check_blocks(H * (r / 128), op), t_blocks = check_blocks(B * nhb * ns, op);
-  const int64_t p_blocks = check_blocks(H * ((B + 31) / 32), op);
+  const int64_t a_blocks = check_blocks(H * (r / 128), op), t_blocks = check_blocks(2 * B * nhb * ns, op) / 2;
+  const int64_t p_blocks = check_blocks(H * ((B + kProjectRows - 1) / kProjectRows), op);
   auto stream = c10::hip::getCurrentHIPStream();
   DLGM_DISPATCH_16(q.scalar_type(), E, {
     LatentArgs<E> p{};
@@ -502,11 +586,11 @@ at::Tensor dlgm_latent_attn_decode(const at::Tensor& q, const at::Tensor& cache,
       constexpr int R = decltype(rc)::value;
       if (dn == 128) {
         latent_absorb_kernel<E, 128><<<a_blocks, kThreads, 0, stream>>>(p, R);
-        latent_attend_kernel<E, R, 64><<<t_blocks, kThreads, 0, stream>>>(p);
+        latent_attend_kernel<E, R, 64><<<t_blocks, kLatentThreads, 0, stream>>>(p);
         latent_project_kernel<E, R, 128><<<p_blocks, kThreads, 0, stream>>>(p);
       } else {
         latent_absorb_kernel<E, 64><<<a_blocks, kThreads, 0, stream>>>(p, R);
-        latent_attend_kernel<E, R, 32><<<t_blocks, kThreads, 0, stream>>>(p);
+        latent_attend_kernel<E, R, 32><<<t_blocks, kLatentThreads, 0, stream>>>(p);
         latent_project_kernel<E, R, 64><<<p_blocks, kThreads, 0, stream>>>(p);
       }
     };
@@ -543,11 +627,10 @@ at::Tensor dlgm_prefix_attn_decode(const at::Tensor& q, const at::Tensor& k, con
   const c10::DeviceGuard guard(q.device());
   auto out = at::empty({B, Hq, D}, q.options());
   if (B == 0 || Hq == 0) return out;
-  const int64_t rep = Hq / Hkv, n = B / G, psteps = (P + 127) / 128, osteps = (L + 127) / 128;
+  const int64_t rep = Hq / Hkv, n = B / G, psteps = (P + kStep - 1) / kStep, osteps = (L + kStep - 1) / kStep;
   const int prw = row_waves(n * rep), orw = row_waves(rep);
   const int64_t prb = (n * rep + 32 * prw - 1) / (32 * prw), orb = (rep + 32 * orw - 1) / (32 * orw);
-  // both kinds of workgroup get about the same number of steps, 1024 workgroups in all (256 at a time: the tiles fill a
-  // CU's LDS)
+  // both kinds of workgroup get about the same number of steps, 1024 workgroups in all, of which 512 run at a time
   const int64_t pitems = G * Hkv * prb, oitems = B * Hkv * orb;
   const int64_t per = std::max<int64_t>(1, (pitems * psteps + oitems * osteps + 1023) / 1024);
   const int64_t np = P ? parts_of(psteps, 1, (psteps + per - 1) / per) : 0;
