@@ -57,8 +57,9 @@ struct SharedArgs {
   float scale, scale_log2, neg_inv_scale;
   bool causal;
 
-  __device__ __forceinline__ int len(int b) const { return lens ? min(max(lens[b], 0), S) : S; }
-  __device__ __forceinline__ int plen(int g) const { return plens ? min(max(plens[g], 0), P) : P; }
+  // the length of b (g), in a scalar register
+  __device__ __forceinline__ int len(int b) const { return lens ? clamp_len(lens[b], S) : S; }
+  __device__ __forceinline__ int plen(int g) const { return plens ? clamp_len(plens[g], P) : P; }
 };
 
 // ---- forward: one workgroup per (b, q head, 128 queries)
@@ -85,6 +86,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_fwd_kernel(SharedArgs<E> p
   vec8_t<E> qf[KK];
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) qf[kk] = row8(qb + (int64_t)qcol * p.q_ss + 16 * kk + 8 * h, qcol < len);
+  settle(qf);
 
   const E* kb = p.k + b * p.k_sb + hk * p.k_sh;
   const E* vb = p.v + b * p.v_sb + hk * p.v_sh;
@@ -246,6 +248,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_bwd_dq_kernel(SharedArgs<E
       p.rows[(int64_t)p.B * p.Hq * p.S + rowc] = in ? p.lse[rowc] * p.neg_inv_scale : 0.f;
     }
   }
+  settle(qf), settle(dof);
 
   const E* kb = p.k + b * p.k_sb + hk * p.k_sh;
   const E* vb = p.v + b * p.v_sb + hk * p.v_sh;
@@ -385,6 +388,7 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_bwd_dkdv_kernel(SharedArgs
   vec8_t<E> kf[KK];
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) kf[kk] = row8(kb + (int64_t)key * k_ss + 16 * kk + 8 * h, key < nkeys);
+  settle(kf);
   const RowTile<E, D, kBQ, 0> vt(w, lane);
   vt.issue(vimg, vb + (int64_t)k0 * v_ss, v_ss, nkeys - k0, w);
 
@@ -420,9 +424,11 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_bwd_dkdv_kernel(SharedArgs
     E* img = smem + buf * SLOT;
     qd.issue(img, qb, p.q_ss, c.len - q0, w);
     qd.issue(img + TA, p.dout + c.b * p.do_sb + hd * p.do_sh + (int64_t)q0 * p.do_ss, p.do_ss, c.len - q0, w);
-    if (w == 0) {
-      const int q = min(q0 + (lane & 31), p.S - 1);  // rows past the length hold 0, 0 (and are masked)
-      glds4(p.rows + (lane < 32 ? nrow : 0) + ((int64_t)c.b * p.Hq + hd) * p.S + q, &rc[buf][0]);
+    if (w == 0) {  // the rows' terms: lanes 0 .. 31 -lse/scale, 32 .. 63 -delta
+      const float* rows = p.rows + ((int64_t)c.b * p.Hq + hd) * p.S + q0;
+      const int bytes = 4 * (p.S - q0);
+      if (lane < 32) dma4_async(rows + nrow, bytes, 4 * lane, lds_at(&rc[buf][0]));
+      else dma4_async(rows, bytes, 4 * (lane - 32), lds_at(&rc[buf][0]));
     }
   };
 
@@ -541,8 +547,8 @@ __global__ __launch_bounds__(kKvThreads, 2) void latent_bwd_dkdv_kernel(SharedAr
     qa.issue(img, qb + (int64_t)q0 * p.q_ss, p.q_ss, len - q0, w);
     qr.issue(img + TA, qb + (int64_t)q0 * p.q_ss + DA, p.q_ss, len - q0, w);
     da.issue(img + TA + TB, dob + (int64_t)q0 * p.do_ss, p.do_ss, len - q0, w);
-    // the rows' terms (rows past the length hold 0, 0 and are masked)
-    if (w < 2) glds4(rowb + min(q0 + lane, p.S - 1), &rc[buf][w * kBQ2]);
+    // the rows' terms (past the length 0, 0; those scores are masked)
+    if (w < 2) dma4_async(rowb + q0, 4 * (p.S - q0), 4 * lane, lds_at(&rc[buf][w * kBQ2]));
   };
   // both kinds of wave take the same walk: at tile t, tiles t - 1 and t are in LDS while t + 1 arrives, three buffers.
   // first(buffer of t, of t - 1, t, whether t and t - 1 have work for these keys), second(buffer of t, whether)
@@ -573,6 +579,7 @@ __global__ __launch_bounds__(kKvThreads, 2) void latent_bwd_dkdv_kernel(SharedAr
     const E* krb = p.kr + b * p.kr_sb + (int64_t)key * p.kr_ss + 8 * h;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) kf[kk] = row8(kk < KA ? kb + 16 * kk : krb + 16 * (kk - KA), key < len);
+    settle(kf);
     f32x16 dv[DTV];  // dV^T: [d][key]
 #pragma unroll
     for (int dt = 0; dt < DTV; ++dt) dv[dt] = (f32x16)(0.f);
@@ -632,6 +639,7 @@ __global__ __launch_bounds__(kKvThreads, 2) void latent_bwd_dkdv_kernel(SharedAr
     const E* vb = p.v + b * p.v_sb + hd * p.v_sh + (int64_t)key * p.v_ss + 8 * h;
 #pragma unroll
     for (int kk = 0; kk < KV; ++kk) vf[kk] = row8(vb + 16 * kk, key < len);
+    settle(vf);
     f32x16 dk[DTK];  // dK^T: [d][key]
 #pragma unroll
     for (int dt = 0; dt < DTK; ++dt) dk[dt] = (f32x16)(0.f);

@@ -40,7 +40,7 @@ struct LatentArgs {
   int B, H, L, dn, dv, ns;
   float scale_log2;
 
-  __device__ __forceinline__ int len(int b) const { return min(max(lens[b], 0), L); }
+  __device__ __forceinline__ int len(int b) const { return clamp_len(lens[b], L); }
 };
 
 // qa[b, h, :] = q_nope[b, h, :] W_k[h]: one workgroup per (head, 128 latent columns), a wave per 32 of them, 32 sequences
@@ -136,6 +136,7 @@ __global__ __launch_bounds__(kLatentThreads, 2) void latent_attend_kernel(Latent
         const int kk = KD * KH + j;
         qf[j] = row8(kk < KR ? qa + 16 * kk : qr + 16 * (kk - KR), head < p.H);
       }
+      settle(qf);
     }
     RowFrag<128, 1> cf0(r, h);
     RowFrag<DR, 0> rf0(r, h);
@@ -358,7 +359,7 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_attend_kernel(PrefixArgs<E
     hk = x % p.Hkv;
     const int g = x / p.Hkv;
     b0 = g * p.n, nrows = p.n * rep;
-    len = p.plens ? min(max(p.plens[g], 0), p.P) : p.P;
+    len = p.plens ? clamp_len(p.plens[g], p.P) : p.P;
     kb = p.pk + g * p.pk_sb + hk * p.pk_sh, vb = p.pv + g * p.pv_sb + hk * p.pv_sh;
     k_ss = p.pk_ss, v_ss = p.pv_ss;
   } else {
@@ -368,7 +369,7 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_attend_kernel(PrefixArgs<E
     part = x % p.no, x /= p.no;
     hk = x % p.Hkv;
     b0 = x / p.Hkv, nrows = rep;
-    len = min(max(p.lens[b0], 0), p.L);
+    len = clamp_len(p.lens[b0], p.L);
     kb = p.k + b0 * p.k_sb + hk * p.k_sh, vb = p.v + b0 * p.v_sb + hk * p.v_sh;
     k_ss = p.k_ss, v_ss = p.v_ss;
   }
@@ -381,6 +382,7 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_attend_kernel(PrefixArgs<E
   vec8_t<E> qf[KK];
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) qf[kk] = row8(p.q + seq * p.q_sb + hq * p.q_sh + 16 * kk + 8 * h, ok);
+  settle(qf);
   const RowTile<E, D, kStep, 0> kt(w, lane);
   const RowTile<E, D, kStep, 2> vt(w, lane);
   auto stage = [&](int buf, int t) {
