@@ -129,6 +129,8 @@ def latent_attention(q: torch.Tensor, c: torch.Tensor, k_rope: torch.Tensor, w_k
             or w_kv.shape[0] % max(H, 1) or w_kv.shape[0] <= H * (d - k_rope.shape[-1]):
         raise ValueError(f"latent_attention: q {tuple(q.shape)}, c {tuple(c.shape)}, k_rope {tuple(k_rope.shape)} and "
                          f"w_kv {tuple(w_kv.shape)} do not fit together")
+    if use_native(q):  # the same composition as one operator each way (csrc/autograd.cpp)
+        return hip_ops().latent_attention(q, c, k_rope, w_kv, _scale(q, softmax_scale), causal, lens)
     return LatentAttentionFunction.apply(q, c, k_rope, w_kv, softmax_scale, causal, lens)
 
 

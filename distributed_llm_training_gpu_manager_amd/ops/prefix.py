@@ -118,6 +118,9 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prefix_k
                      softmax_scale: Optional[float] = None, causal: bool = True, lens: Lens = None,
                      prefix_lens: Lens = None) -> torch.Tensor:
     """out [B, S, Hq, D] as :func:`prefix_attn_fwd`, differentiable in q, k, v, prefix_k and prefix_v."""
+    _check(q, k, prefix_k)
+    if use_native(q):  # one operator each way (csrc/autograd.cpp)
+        return hip_ops().prefix_attention(q, k, v, prefix_k, prefix_v, _scale(q, softmax_scale), causal, lens, prefix_lens)
     return PrefixAttentionFunction.apply(q, k, v, prefix_k, prefix_v, softmax_scale, causal, lens, prefix_lens)
 
 

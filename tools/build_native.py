@@ -4,7 +4,7 @@
 Two libraries are produced next to the Python package:
 
 * ``_dlgm_hip.so``  -- the HIP kernels (csrc/kernels/*.hip) + TORCH_LIBRARY
-  registrations (csrc/bindings.cpp), loaded with ``torch.ops.load_library``;
+  registrations (csrc/*.cpp), loaded with ``torch.ops.load_library``;
 * ``_dlgm_host.so`` -- the host runtime (csrc/host/*.cpp): multi-threaded
   checkpoint writer/reader with CRC32C, AVX2/FMA CPU AdamW (ZeRO-Offload). Plain
   C++ built with g++ (no HIP, no torch), driven through ``ctypes``.
@@ -124,7 +124,7 @@ def build(jobs: int | None = None, verbose: bool = False, force: bool = False) -
               "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
     torch_flags = [*common, *(f"-I{p}" for p in tinc), f"-I{sysconfig.get_paths()['include']}",
                    f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DUSE_ROCM=1", "-DTORCH_API_INCLUDE_EXTENSION_H"]
-    kern_src = sorted((CSRC / "kernels").glob("*.hip")) + [CSRC / "bindings.cpp"]
+    kern_src = sorted((CSRC / "kernels").glob("*.hip")) + sorted(CSRC.glob("*.cpp"))
     kern_ld = [f"-L{tlib}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch", "-lhipblaslt",
                f"-Wl,-rpath,{tlib}"]
     outs = [_build_lib("_dlgm_hip.so", kern_src, torch_flags, kern_ld, jobs, verbose, force)]
