@@ -83,11 +83,6 @@ __global__ __launch_bounds__(kThreads, 2) void shared_fwd_kernel(SharedArgs<E> p
   const int len = p.len(b);
   const int q0 = qt * kBQ, q0w = q0 + 32 * w, qcol = q0w + r;
   const E* qb = p.q + b * p.q_sb + hq * p.q_sh;
-  vec8_t<E> qf[KK];
-#pragma unroll
-  for (int kk = 0; kk < KK; ++kk) qf[kk] = row8(qb + (int64_t)qcol * p.q_ss + 16 * kk + 8 * h, qcol < len);
-  settle(qf);
-
   const E* kb = p.k + b * p.k_sb + hk * p.k_sh;
   const E* vb = p.v + b * p.v_sb + hk * p.v_sh;
   const E* krb = DB ? p.kr + b * p.kr_sb : nullptr;
@@ -115,6 +110,11 @@ __global__ __launch_bounds__(kThreads, 2) void shared_fwd_kernel(SharedArgs<E> p
     }
   };
 
+  if (nt > 0) stage(0, 0);  // on its way beside the q fragments
+  vec8_t<E> qf[KK];
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) qf[kk] = row8(qb + (int64_t)qcol * p.q_ss + 16 * kk + 8 * h, qcol < len);
+  settle(qf);
   f32x16 o[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) o[dt] = (f32x16)(0.f);
@@ -187,7 +187,6 @@ __global__ __launch_bounds__(kThreads, 2) void shared_fwd_kernel(SharedArgs<E> p
         for (int s2 = 0; s2 < 2; ++s2)
           o[dt] = mfma32(vf.read(vi, dt, 32 * u + 16 * s2), pf[u][s2], o[dt]);
   };
-  if (nt > 0) stage(0, 0);
   for (int t = 0; t < nt; t += 2) {
     tile(std::integral_constant<int, 0>{}, t);
     if (t + 1 < nt) tile(std::integral_constant<int, 1>{}, t + 1);
@@ -221,6 +220,34 @@ __global__ __launch_bounds__(kThreads, 2) void shared_bwd_dq_kernel(SharedArgs<E
   const int len = p.len(b);
   const int q0 = qt * kBQ, q0w = q0 + 32 * w, qcol = q0w + r;
   const bool in = qcol < len;
+  const E* kb = p.k + b * p.k_sb + hk * p.k_sh;
+  const E* vb = p.v + b * p.v_sb + hk * p.v_sh;
+  const E* krb = DB ? p.kr + b * p.kr_sb : nullptr;
+  const E* pkb = PRE ? p.pk + grp * p.pk_sb + hk * p.pk_sh : nullptr;
+  const E* pvb = PRE ? p.pv + grp * p.pv_sb + hk * p.pv_sh : nullptr;
+  const int plen = PRE ? p.plen(grp) : 0;
+  const int np = (plen + kBKV - 1) / kBKV;
+  const int kv_end = p.causal ? min(len, q0 + kBQ) : len;
+  const int nt = q0 < len ? np + (kv_end + kBKV - 1) / kBKV : 0;
+
+  const RowTile<E, DA, kBKV, 1> ka(w, lane);
+  const RowTile<E, DBX, kBKV, 1> kr(w, lane);
+  const RowTile<E, DV, kBKV, 0> va(w, lane);
+  auto stage = [&](int buf, int t) {
+    E* img = smem + buf * SLOT;
+    if (PRE && t < np) {
+      const int row0 = t * kBKV;
+      ka.issue(img, pkb + (int64_t)row0 * p.pk_ss, p.pk_ss, plen - row0, w);
+      va.issue(img + TA + TB, pvb + (int64_t)row0 * p.pv_ss, p.pv_ss, plen - row0, w);
+    } else {
+      const int row0 = (t - np) * kBKV;
+      ka.issue(img, kb + (int64_t)row0 * p.k_ss, p.k_ss, len - row0, w);
+      if constexpr (DB > 0) kr.issue(img + TA, krb + (int64_t)row0 * p.kr_ss, p.kr_ss, len - row0, w);
+      va.issue(img + TA + TB, vb + (int64_t)row0 * p.v_ss, p.v_ss, len - row0, w);
+    }
+  };
+
+  if (nt > 0) stage(0, 0);  // on its way beside the q and dO fragments
   const E* qb = p.q + b * p.q_sb + hq * p.q_sh + (int64_t)qcol * p.q_ss;
   const E* dob = p.dout + b * p.do_sb + hq * p.do_sh + (int64_t)qcol * p.do_ss;
   vec8_t<E> qf[KK], dof[KV];
@@ -249,34 +276,6 @@ __global__ __launch_bounds__(kThreads, 2) void shared_bwd_dq_kernel(SharedArgs<E
     }
   }
   settle(qf), settle(dof);
-
-  const E* kb = p.k + b * p.k_sb + hk * p.k_sh;
-  const E* vb = p.v + b * p.v_sb + hk * p.v_sh;
-  const E* krb = DB ? p.kr + b * p.kr_sb : nullptr;
-  const E* pkb = PRE ? p.pk + grp * p.pk_sb + hk * p.pk_sh : nullptr;
-  const E* pvb = PRE ? p.pv + grp * p.pv_sb + hk * p.pv_sh : nullptr;
-  const int plen = PRE ? p.plen(grp) : 0;
-  const int np = (plen + kBKV - 1) / kBKV;
-  const int kv_end = p.causal ? min(len, q0 + kBQ) : len;
-  const int nt = q0 < len ? np + (kv_end + kBKV - 1) / kBKV : 0;
-
-  const RowTile<E, DA, kBKV, 1> ka(w, lane);
-  const RowTile<E, DBX, kBKV, 1> kr(w, lane);
-  const RowTile<E, DV, kBKV, 0> va(w, lane);
-  auto stage = [&](int buf, int t) {
-    E* img = smem + buf * SLOT;
-    if (PRE && t < np) {
-      const int row0 = t * kBKV;
-      ka.issue(img, pkb + (int64_t)row0 * p.pk_ss, p.pk_ss, plen - row0, w);
-      va.issue(img + TA + TB, pvb + (int64_t)row0 * p.pv_ss, p.pv_ss, plen - row0, w);
-    } else {
-      const int row0 = (t - np) * kBKV;
-      ka.issue(img, kb + (int64_t)row0 * p.k_ss, p.k_ss, len - row0, w);
-      if constexpr (DB > 0) kr.issue(img + TA, krb + (int64_t)row0 * p.kr_ss, p.kr_ss, len - row0, w);
-      va.issue(img + TA + TB, vb + (int64_t)row0 * p.v_ss, p.v_ss, len - row0, w);
-    }
-  };
-
   f32x16 dqt[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) dqt[dt] = (f32x16)(0.f);
@@ -329,7 +328,6 @@ __global__ __launch_bounds__(kThreads, 2) void shared_bwd_dq_kernel(SharedArgs<E
         }
     }
   };
-  if (nt > 0) stage(0, 0);
   for (int t = 0; t < nt; t += 2) {
     tile(std::integral_constant<int, 0>{}, t);
     if (t + 1 < nt) tile(std::integral_constant<int, 1>{}, t + 1);

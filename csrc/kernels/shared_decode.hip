@@ -126,6 +126,7 @@ __global__ __launch_bounds__(kLatentThreads, 2) void latent_attend_kernel(Latent
 
   auto walk = [&](auto kdc) {
     constexpr int KD = decltype(kdc)::value;
+    if (t0 < t1) stage(0, t0);  // on its way beside the q fragments
     const int head = head0 + 32 * hb + r;
     vec8_t<E> qf[KH];
     {
@@ -143,7 +144,6 @@ __global__ __launch_bounds__(kLatentThreads, 2) void latent_attend_kernel(Latent
     TrFrag<128, 1> vf0(h, i16, g4);
     float* const mine = xbuf[2 * (2 * KD + hb) + u];
     float* const theirs = xbuf[2 * (2 * (1 - KD) + hb) + u];
-    if (t0 < t1) stage(0, t0);
     for (int t = t0, buf = 0; t < t1; ++t, buf ^= 1) {
       vm_drain();
       __syncthreads();
@@ -262,54 +262,92 @@ __global__ __launch_bounds__(kLatentThreads, 2) void latent_attend_kernel(Latent
   }
 }
 
-// One workgroup per (head, 8 sequences): a wave joins the parts of two of them into the latent output, then out = W_v[h] o.
-// The latent output enters its product as two 16-bit terms (value and remainder), so it is not rounded: the product is a
-// small part of the call.
-constexpr int kProjectRows = 8;
+// One workgroup per (head, 8 sequences): join the parts into the latent outputs, then out = W_v[h] o. What another XCD has
+// just written takes some 3 us to arrive (measured: one more round of part loads adds that), so everything is asked for at
+// once: every wave takes one sequence's parts, or, for few sequences, a share of them, and its piece of W_v. The latent
+// output enters its product as two 16-bit terms (value and remainder), so it is not rounded: the product is a small part
+// of the call.
+constexpr int kProjectRows = 8, kProjectThreads = 512;
 template <typename E, int R, int DV>
-__global__ __launch_bounds__(kThreads) void latent_project_kernel(LatentArgs<E> p) {
-  constexpr int LD = R + 8;
+__global__ __launch_bounds__(kProjectThreads) void latent_project_kernel(LatentArgs<E> p) {
+  constexpr int LD = R + 8, TILES = DV / 32, KP = 8 / TILES, KS = R / 16 / KP;  // column tiles, shares of r, k-steps of one
+  constexpr int BATCH = 8;  // parts in flight
+  __shared__ __attribute__((aligned(16))) float red[8][R];  // by wave; then the products' shares
   __shared__ __attribute__((aligned(16))) E ol[2][kProjectRows * LD];
+  static_assert(8 * 2 * 8 * 16 <= 8 * R, "the shares fit");
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 31, h = lane >> 5;
   const int work = xcd_remap(blockIdx.x, gridDim.x), nb = (p.B + kProjectRows - 1) / kProjectRows;
   const int head = work / nb, b0 = work % nb * kProjectRows;  // workgroups of one head read the same W_v
-  const int col = lane * 8 % R;  // r 256: the upper lanes repeat the lower (readlane below needs all of them to run)
-  for (int k = w; k < kProjectRows; k += 4) {
-    const int b = b0 + k;
-    f32x8 acc = (f32x8)(0.f);
-    if (b < p.B) {
-      const int64_t slot = ((int64_t)b * p.H + head) * p.ns;
-      float ms = -INFINITY, ls = 0.f;  // of part `lane` (at most 64 parts)
-      if (lane < p.ns) ms = p.ml[2 * (slot + lane)], ls = p.ml[2 * (slot + lane) + 1];
-      const float m = wave_max(ms);
-      float f = ls == 0.f ? 0.f : fast_exp2(ms - m);  // an empty part (a NaN sum is none)
-      const float l = wave_sum(f * ls);
-      f = l == 0.f ? 0.f : f / l;  // a sequence without keys: zeros
-#pragma unroll 4
-      for (int s = 0; s < p.ns; ++s) {
-        const float fs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s));
-        if (fs == 0.f) continue;  // nothing was written there
-        acc += load8(p.o + (slot + s) * R + col) * fs;
-      }
+  const int rows = min(kProjectRows, p.B - b0);
+  const int lg = rows > 4 ? 3 : rows > 2 ? 2 : rows > 1 ? 1 : 0, share = 8 >> lg;  // waves of a sequence
+  const int seq = min(w >> (3 - lg), rows - 1), first = w & (share - 1);  // waves past the batch repeat its last sequence
+
+  const int64_t slot = ((int64_t)(b0 + seq) * p.H + head) * p.ns;
+  const float* ml = p.ml + 2 * slot;
+  const int col = lane * 8 % R;  // r 256: the upper lanes repeat the lower
+  const float* o = p.o + slot * R + col;
+  f32x8 x[BATCH], acc = (f32x8)(0.f);
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int s = 0; s < BATCH; ++s) x[s] = load8(o + min(s0 + s * share, p.ns - 1) * R);
+  };
+  load(first);
+  const int tile = w % TILES, k0 = w / TILES * KS;
+  const E* wv = p.w + ((int64_t)head * (p.dn + p.dv) + p.dn + 32 * tile + r) * p.w_ss + 16 * k0 + 8 * h;
+  vec8_t<E> wf[KS];
+#pragma unroll
+  for (int kk = 0; kk < KS; ++kk) wf[kk] = *reinterpret_cast<const vec8_t<E>*>(wv + 16 * kk);
+  float m = -INFINITY, l = 0.f;  // of the sequence, the same in every lane
+#pragma unroll 8
+  for (int s = 0; s < p.ns; ++s) m = fmaxf(m, ml[2 * s]);
+#pragma unroll 8
+  for (int s = 0; s < p.ns; ++s) l += ml[2 * s + 1] == 0.f ? 0.f : fast_exp2(ml[2 * s] - m) * ml[2 * s + 1];
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // a sequence without keys: zeros
+  for (int s0 = first; s0 < p.ns; s0 += BATCH * share) {
+    if (s0 > first) load(s0);
+#pragma unroll
+    for (int s = 0; s < BATCH; ++s) {
+      const int k = s0 + s * share, kc = min(k, p.ns - 1);
+      // an empty part (a NaN sum is none): nothing was written there
+      const float f = k < p.ns && ml[2 * kc + 1] != 0.f ? fast_exp2(ml[2 * kc] - m) * inv : 0.f;
+      acc += f == 0.f ? (f32x8)(0.f) : x[s] * f;
     }
-    const vec8_t<E> hi = __builtin_convertvector(acc, vec8_t<E>);
-    *reinterpret_cast<vec8_t<E>*>(ol[0] + k * LD + col) = hi;
-    store8f(ol[1] + k * LD + col, acc - __builtin_convertvector(hi, f32x8));
+  }
+  *reinterpret_cast<f32x8*>(&red[w][col]) = acc;
+  __syncthreads();
+  for (int i = threadIdx.x * 8; i < rows * R; i += kProjectThreads * 8) {
+    const int k = i / R, c = i % R;
+    f32x8 v = load8(&red[k * share][c]);
+    for (int j = 1; j < share; ++j) v += load8(&red[k * share + j][c]);
+    const vec8_t<E> hi = __builtin_convertvector(v, vec8_t<E>);
+    *reinterpret_cast<vec8_t<E>*>(ol[0] + k * LD + c) = hi;
+    store8f(ol[1] + k * LD + c, v - __builtin_convertvector(hi, f32x8));
   }
   __syncthreads();
-  if (w >= DV / 32) return;
-  const E* wv = p.w + ((int64_t)head * (p.dn + p.dv) + p.dn + 32 * w + r) * p.w_ss + 8 * h;
-  const int at = r % kProjectRows * LD + 8 * h;  // columns past the sequences repeat them and are not stored
-  f32x16 acc = (f32x16)(0.f);
-#pragma unroll 16
-  for (int kk = 0; kk < R / 16; ++kk) {
-    const vec8_t<E> a = *reinterpret_cast<const vec8_t<E>*>(wv + 16 * kk);
-    acc = mfma32(a, lds_read_b128(ol[0] + at + 16 * kk), acc);
-    acc = mfma32(a, lds_read_b128(ol[1] + at + 16 * kk), acc);
+  const int at = r % kProjectRows * LD + 16 * k0 + 8 * h;  // columns past the sequences are not stored
+  f32x16 out[2] = {(f32x16)(0.f), (f32x16)(0.f)};
+#pragma unroll
+  for (int kk = 0; kk < KS; ++kk)
+#pragma unroll
+    for (int y = 0; y < 2; ++y) out[y] = mfma32(wf[kk], lds_read_b128(ol[y] + at + 16 * kk), out[y]);
+  out[0] += out[1];
+  float* mine = &red[0][0] + ((w * 2 + h) * 8 + r) * 16;  // red has been read
+  if (r < 8) {
+#pragma unroll
+    for (int j = 0; j < 16; j += 8)
+      *reinterpret_cast<f32x8*>(mine + j) = (f32x8){out[0][j], out[0][j + 1], out[0][j + 2], out[0][j + 3],
+                                                    out[0][j + 4], out[0][j + 5], out[0][j + 6], out[0][j + 7]};
   }
-  const f32x16 acc1[1] = {acc};
-  store_rows_bf16<1>(p.out + ((int64_t)(b0 + r) * p.H + head) * DV + 32 * w, acc1, 1.f, h, r < kProjectRows && b0 + r < p.B);
+  __syncthreads();
+  if (w >= TILES) return;
+  f32x16 sum[1] = {(f32x16)(0.f)};
+  for (int k = 0; k < KP; ++k) {
+    const float* from = &red[0][0] + (((w + k * TILES) * 2 + h) * 8 + r % 8) * 16;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) sum[0][j] += from[j];
+  }
+  store_rows_bf16<1>(p.out + ((int64_t)(b0 + r) * p.H + head) * DV + 32 * w, sum, 1.f, h, r < rows);
 }
 
 // ---- shared prefix ------------------------------------------------------------------------------
@@ -379,10 +417,6 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_attend_kernel(PrefixArgs<E
   const int steps = (len + kStep - 1) / kStep;
   const int t0 = (int)((int64_t)steps * part / nparts), t1 = (int)((int64_t)steps * (part + 1) / nparts);
 
-  vec8_t<E> qf[KK];
-#pragma unroll
-  for (int kk = 0; kk < KK; ++kk) qf[kk] = row8(p.q + seq * p.q_sb + hq * p.q_sh + 16 * kk + 8 * h, ok);
-  settle(qf);
   const RowTile<E, D, kStep, 0> kt(w, lane);
   const RowTile<E, D, kStep, 2> vt(w, lane);
   auto stage = [&](int buf, int t) {
@@ -390,6 +424,11 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_attend_kernel(PrefixArgs<E
     kt.issue(img, kb + (int64_t)t * kStep * k_ss, k_ss, len - t * kStep, w);
     vt.issue(img + TI, vb + (int64_t)t * kStep * v_ss, v_ss, len - t * kStep, w);
   };
+  if (t0 < t1) stage(0, t0);  // on its way beside the q fragments
+  vec8_t<E> qf[KK];
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) qf[kk] = row8(p.q + seq * p.q_sb + hq * p.q_sh + 16 * kk + 8 * h, ok);
+  settle(qf);
   f32x16 o[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) o[dt] = (f32x16)(0.f);
@@ -446,7 +485,6 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_attend_kernel(PrefixArgs<E
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2) o[dt] = mfma32(vf.read(vi, dt, 32 * u + 16 * s2), pf[u][s2], o[dt]);
   };
-  if (t0 < t1) stage(0, t0);
   for (int t = t0; t < t1; ++t) {
     vm_drain();
     __syncthreads();
@@ -518,12 +556,14 @@ __global__ __launch_bounds__(kThreads) void prefix_join_kernel(PrefixArgs<E> p) 
   for (int x = 0; x < 2; ++x) {
     const float f = ls[x] == 0.f ? 0.f : fast_exp2(ms[x] - m);  // an empty part (a NaN sum is none)
     l += f * ls[x];
-#pragma unroll 4
-    for (int s = 64 * x + w; s < min(slots, 64 * x + 64); s += 4) {
+#pragma unroll 8
+    for (int s = 64 * x + w; s < min(slots, 64 * x + 64); s += 4) {  // loads without a branch: eight in flight
       const float fs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s & 63));
-      if (fs == 0.f) continue;  // nothing was written there
+      float o[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) acc[j] += fs * p.o[(base + s) * D + lane * V + j];
+      for (int j = 0; j < V; ++j) o[j] = p.o[(base + s) * D + lane * V + j];
+#pragma unroll
+      for (int j = 0; j < V; ++j) acc[j] += fs == 0.f ? 0.f : fs * o[j];  // nothing was written to an empty part
     }
   }
   l = wave_sum(l);
@@ -575,7 +615,7 @@ at::Tensor dlgm_latent_attn_decode(const at::Tensor& q, const at::Tensor& cache,
   auto o = at::empty({B, H, ns, r}, q.options().dtype(at::kFloat));
   auto ml = at::empty({B, H, ns, 2}, q.options().dtype(at::kFloat));
   const int64_t a_blocks = check_blocks(H * (r / 128), op), t_blocks = check_blocks(2 * B * nhb * ns, op) / 2;
-  const int64_t p_blocks = check_blocks(H * ((B + kProjectRows - 1) / kProjectRows), op);
+  const int64_t p_blocks = check_blocks(2 * H * ((B + kProjectRows - 1) / kProjectRows), op) / 2;
   auto stream = c10::hip::getCurrentHIPStream();
   DLGM_DISPATCH_16(q.scalar_type(), E, {
     LatentArgs<E> p{};
@@ -589,11 +629,11 @@ at::Tensor dlgm_latent_attn_decode(const at::Tensor& q, const at::Tensor& cache,
       if (dn == 128) {
         latent_absorb_kernel<E, 128><<<a_blocks, kThreads, 0, stream>>>(p, R);
         latent_attend_kernel<E, R, 64><<<t_blocks, kLatentThreads, 0, stream>>>(p);
-        latent_project_kernel<E, R, 128><<<p_blocks, kThreads, 0, stream>>>(p);
+        latent_project_kernel<E, R, 128><<<p_blocks, kProjectThreads, 0, stream>>>(p);
       } else {
         latent_absorb_kernel<E, 64><<<a_blocks, kThreads, 0, stream>>>(p, R);
         latent_attend_kernel<E, R, 32><<<t_blocks, kLatentThreads, 0, stream>>>(p);
-        latent_project_kernel<E, R, 64><<<p_blocks, kThreads, 0, stream>>>(p);
+        latent_project_kernel<E, R, 64><<<p_blocks, kProjectThreads, 0, stream>>>(p);
       }
     };
     if (r == 512) run(std::integral_constant<int, 512>{});
@@ -634,7 +674,7 @@ at::Tensor dlgm_prefix_attn_decode(const at::Tensor& q, const at::Tensor& k, con
   const int64_t prb = (n * rep + 32 * prw - 1) / (32 * prw), orb = (rep + 32 * orw - 1) / (32 * orw);
   // both kinds of workgroup get about the same number of steps, 1024 workgroups in all, of which 512 run at a time
   const int64_t pitems = G * Hkv * prb, oitems = B * Hkv * orb;
-  const int64_t per = std::max<int64_t>(1, (pitems * psteps + oitems * osteps + 1023) / 1024);
+  const int64_t per = std::max<int64_t>(1, (pitems * psteps + oitems * osteps + 511) / 512);
   const int64_t np = P ? parts_of(psteps, 1, (psteps + per - 1) / per) : 0;
   const int64_t no = L ? parts_of(osteps, 1, (osteps + per - 1) / per) : 0;
   if (np + no == 0) return out.zero_();
