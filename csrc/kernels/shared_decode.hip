@@ -76,27 +76,39 @@ __global__ __launch_bounds__(kThreads) void latent_absorb_kernel(LatentArgs<E> p
 }
 
 // One workgroup per (sequence, 64 heads, part of its length): tiles of 64 cache rows by LDS-DMA, one ahead (two tiles fill a
-// CU's LDS, so its 8 waves are two a SIMD). Scores: the waves (u, hb, kd) take 32 rows x 32 heads over half of the r + dr
-// columns each, q in registers; the halves meet in LDS, where each of a pair keeps 16 of the 32 rows: their weights go back
-// to LDS as matrix operands. Outputs: each wave takes r / 8 latent columns of all 64 heads. 64 heads a workgroup keep LDS
-// reads (every wave reads 32 rows of half the columns: 147 KiB a tile, 64 KiB of it again transposed) beside the matrix
-// products (68 a SIMD). With 4 waves over whole rows, one a SIMD, 128 heads over 32 x 16384 tokens took 300 us.
+// CU's LDS, so its 8 waves are two a SIMD). Scores, 16x16x32 products: the waves (kq, hb) take 16 rows x 32 heads each over
+// all r + dr columns, q in registers (144 at r 512) -- every cache row's LDS reads serve 32 heads, and no wave needs
+// another's scores. The weights go through LDS as matrix operands. Outputs, 32x32x16 products: each wave takes r / 8 latent
+// columns of all 64 heads. The running reference of a head is raised only when some wave sees it outgrown by
+// 2^kRescaleLog2, which all learn at the one barrier between weights and outputs.
 constexpr int kLatentThreads = 512;
+
+__device__ __forceinline__ f32x4 mfma16(const bf16x8& a, const bf16x8& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16(const f16x8& a, const f16x8& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+// x of lane i ^ 16
+__device__ __forceinline__ float swap_quarters(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(__lane_id() & 16 ? r[0] : r[1]);
+}
 
 template <typename E, int R, int DR>
 __global__ __launch_bounds__(kLatentThreads, 2) void latent_attend_kernel(LatentArgs<E> p) {
-  constexpr int NI = R / 128, KR = R / 16, KK = KR + DR / 16, KH = KK / 2;  // images, k-steps, a wave's k-steps
+  constexpr int NI = R / 128, KR = R / 32, KK = KR + DR / 32;  // images, k-steps of 32 columns
   constexpr int TI = 64 * 128, SLOT = 64 * (R + DR);
   constexpr int DT = R / 256;  // 32-column output tiles of a wave
-  static_assert(KK % 2 == 0, "the columns split evenly over a pair of waves");
   __shared__ __attribute__((aligned(16))) E smem[2 * SLOT];
-  // 2 KiB a wave: its partner's half of the scores (2 KiB); then, written by the partner, who alone has read them: a
-  // fragment of weights (1 KiB), the maxima of 32 heads and whether one outgrew the reference
-  __shared__ __attribute__((aligned(16))) float xbuf[8][512];
+  __shared__ __attribute__((aligned(16))) E pbuf[4][2][512];  // weights: [16 rows][32 heads] fragments of 64 lanes x 8
+  __shared__ __attribute__((aligned(16))) E qrope[2][DR / 32][512];  // [32 heads][k-step] fragments of the first 16
+  __shared__ float smax[4][64];                              // maxima of 16 rows for 64 heads; at the end, sums
+  __shared__ int grown[8];
 
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 31, h = lane >> 5, i16 = lane & 15, g4 = lane >> 4;
-  const int u = w & 1, hb = (w >> 1) & 1;
+  const int kq = w & 3, hb = w >> 2;
   const int nhb = (p.H + 63) / 64;
   // head blocks of one (sequence, part) read the same rows: they follow each other on one XCD
   const int work = xcd_remap(blockIdx.x, gridDim.x);
@@ -106,148 +118,152 @@ __global__ __launch_bounds__(kLatentThreads, 2) void latent_attend_kernel(Latent
   const int t0 = (int)((int64_t)tiles * part / p.ns), t1 = (int)((int64_t)tiles * (part + 1) / p.ns);
   const int blocks = head0 + 32 < p.H ? 2 : 1;  // of 32 heads that exist
 
-  const RowTile<E, 128, 64, 1, 8> ct(w, lane);
-  const RowTile<E, DR, 64, 0, 8> rt(w, lane);
+  // what a lane derives from its number is derived again for every tile: at r 512 the q fragments and outputs leave no
+  // register to keep it in (13 were spilled, and a spilled register's reload waits for the tile in flight as well)
+  auto here = [&] {
+    int x = lane;
+    pin(x);
+    return x;
+  };
   const E* cb = p.cache + b * p.c_sb;
   auto stage = [&](int buf, int t) {
+    const int ln = here();
+    const RowTile<E, 128, 64, 1, 8> ct(w, ln);
+    const RowTile<E, DR, 64, 0, 8> rt(w, ln);
     E* img = smem + buf * SLOT;
     const E* base = cb + (int64_t)t * 64 * p.c_ss;
 #pragma unroll
     for (int i = 0; i < NI; ++i) ct.issue(img + i * TI, base + 128 * i, p.c_ss, len - t * 64, w);
     rt.issue(img + NI * TI, base + R, p.c_ss, len - t * 64, w);
   };
+  if (t0 < t1) stage(0, t0);  // on its way beside the q fragments
 
+  vec8_t<E> qf[KK + KR];  // [k-step][16 heads]; the first 16 heads' rope columns stay in LDS, as fragments
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int head = head0 + 32 * hb + 16 * x + i16;
+    const E* qa = p.qa + ((int64_t)b * p.H + head) * R + 8 * g4;
+    const E* qr = p.q + b * p.q_sb + head * p.q_sh + p.dn + 8 * g4;
+#pragma unroll
+    for (int kk = 0; kk < KR; ++kk) qf[2 * kk + x] = row8(qa + 32 * kk, head < p.H);
+#pragma unroll
+    for (int kk = 0; kk < KK - KR; ++kk) {
+      const vec8_t<E> f = row8(qr + 32 * kk, head < p.H);
+      if (x) qf[2 * KR + kk] = f;
+      else *reinterpret_cast<vec8_t<E>*>(&qrope[hb][kk][8 * lane]) = f;  // the same from each of the block's four waves
+    }
+  }
+  settle(qf);
   f32x16 o[2][DT];  // [head block][column tile]
 #pragma unroll
   for (int x = 0; x < 2; ++x)
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[x][dt] = (f32x16)(0.f);
-  float m_run[2] = {-INFINITY, -INFINITY}, l_run = 0.f;  // reference of heads r and 32 + r; the sum over this wave's rows
-
-  auto walk = [&](auto kdc) {
-    constexpr int KD = decltype(kdc)::value;
-    if (t0 < t1) stage(0, t0);  // on its way beside the q fragments
-    const int head = head0 + 32 * hb + r;
-    vec8_t<E> qf[KH];
-    {
-      const E* qa = p.qa + ((int64_t)b * p.H + head) * R + 8 * h;
-      const E* qr = p.q + b * p.q_sb + head * p.q_sh + p.dn + 8 * h;
+  // references (log2 domain) of the heads of this lane's scores, 16 x + i16 of block hb, and of its outputs, 32 x + r
+  float m_s[2] = {-INFINITY, -INFINITY}, m_o[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+  for (int t = t0, buf = 0; t < t1; ++t, buf ^= 1) {
+    vm_drain();
+    __syncthreads();
+    if (t + 1 < t1) stage(buf ^ 1, t + 1);
+    const E* img = smem + buf * SLOT;
+    f32x4 s[2] = {(f32x4)(0.f), (f32x4)(0.f)};
+    if (hb < blocks) {
+      // rows of this wave, columns 8 g4 of a 32-column step
+      const int ln = here(), row = 16 * kq + (ln & 15);
+      const int ca = row * 128 + (swz_dual<128>(row, ln >> 4) << 3), ra = NI * TI + row * DR + (swz_row<DR>(row, ln >> 4) << 3);
 #pragma unroll
-      for (int j = 0; j < KH; ++j) {
-        const int kk = KD * KH + j;
-        qf[j] = row8(kk < KR ? qa + 16 * kk : qr + 16 * (kk - KR), head < p.H);
+      for (int kk = 0; kk < KK; ++kk) {
+        const vec8_t<E> a = lds_read_b128(img + (kk < KR ? kk / 4 * TI + (ca ^ (kk % 4 << 5)) : (ra ^ (kk - KR << 5))));
+        s[0] = mfma16(a, kk < KR ? qf[2 * kk] : lds_read_b128(&qrope[hb][kk - KR][8 * ln]), s[0]);
+        s[1] = mfma16(a, kk < KR ? qf[2 * kk + 1] : qf[KR + kk], s[1]);
       }
-      settle(qf);
     }
-    RowFrag<128, 1> cf0(r, h);
-    RowFrag<DR, 0> rf0(r, h);
-    TrFrag<128, 1> vf0(h, i16, g4);
-    float* const mine = xbuf[2 * (2 * KD + hb) + u];
-    float* const theirs = xbuf[2 * (2 * (1 - KD) + hb) + u];
-    for (int t = t0, buf = 0; t < t1; ++t, buf ^= 1) {
-      vm_drain();
+    if (uniform(t * 64 + 64 > len)) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (t * 64 + 16 * kq + 4 * g4 + j >= len) s[0][j] = s[1][j] = -INFINITY;
+    }
+    float mx[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) mx[x] = fmaxf(fmaxf(s[x][0], s[x][1]), fmaxf(s[x][2], s[x][3])) * p.scale_log2;
+    // weights over the references so far: right unless a head outgrew its own, which is seen at the barrier
+    float sum[2];
+    auto weigh = [&] {
+      const int ln = here(), q4 = ln >> 4;
+      E* to = &pbuf[kq][hb][((ln & 15) + 32 * (q4 & 1)) * 8 + 4 * (q4 >> 1)];  // rows 4 g4 .. +3 of head i16
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const float m = m_s[x] == -INFINITY ? 0.f : m_s[x];
+        f32x4 e;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) e[j] = fast_exp2(s[x][j] * p.scale_log2 - m);
+        sum[x] = (e[0] + e[1]) + (e[2] + e[3]);
+        *reinterpret_cast<vec4_t<E>*>(to + 16 * x * 8) = __builtin_convertvector(e, vec4_t<E>);
+      }
+    };
+    weigh();
+    const int big = __any(mx[0] > m_s[0] + kRescaleLog2 || mx[1] > m_s[1] + kRescaleLog2);
+    if (lane == 0) grown[w] = big;
+    __syncthreads();
+    if (__any(grown[lane & 7] != 0)) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        mx[x] = fmaxf(mx[x], swap_quarters(mx[x]));
+        mx[x] = fmaxf(mx[x], swap_halves(mx[x]));
+        if (g4 == 0) smax[kq][32 * hb + 16 * x + i16] = mx[x];
+      }
       __syncthreads();
-      if (t + 1 < t1) stage(buf ^ 1, t + 1);
-      const E* img = smem + buf * SLOT;
-      f32x16 s = (f32x16)(0.f);
-      if (hb < blocks) {
-        RowFrag<128, 1> cf = cf0;
-        RowFrag<DR, 0> rf = rf0;
-        cf.at += 32 * u * 128, rf.at += NI * TI + 32 * u * DR;
-        pin(cf.at), pin(rf.at);
 #pragma unroll
-        for (int j = 0; j < KH; ++j) {
-          const int kk = KD * KH + j;
-          s = mfma32(lds_read_b128(img + (kk < KR ? kk / 8 * TI + cf(kk % 8) : rf(kk - KR))), qf[j], s);
-        }
+      for (int x = 0; x < 2; ++x) {
+        const int hs = 32 * hb + 16 * x + i16, ho = 32 * x + r;
+        const float ns = fmaxf(m_s[x], fmaxf(fmaxf(smax[0][hs], smax[1][hs]), fmaxf(smax[2][hs], smax[3][hs])));
+        const float no = fmaxf(m_o[x], fmaxf(fmaxf(smax[0][ho], smax[1][ho]), fmaxf(smax[2][ho], smax[3][ho])));
+        l_run[x] *= ns == -INFINITY ? 1.f : fast_exp2(m_s[x] - ns);
+        const float alpha = no == -INFINITY ? 1.f : fast_exp2(m_o[x] - no);
+        m_s[x] = ns, m_o[x] = no;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[x][dt] *= alpha;
       }
-      // each of the pair keeps the 16 rows whose scores are registers 8 KD .. 8 KD + 7
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        *reinterpret_cast<f32x4*>(mine + 256 * j + 4 * lane) =
-            (f32x4){s[8 - 8 * KD + 4 * j], s[8 - 8 * KD + 4 * j + 1], s[8 - 8 * KD + 4 * j + 2], s[8 - 8 * KD + 4 * j + 3]};
+      weigh();
       __syncthreads();
-      float v[8];
+    }
+    l_run[0] += sum[0], l_run[1] += sum[1];
+    const int ln = here();
+    const TrFrag<128, 1> vf(ln >> 5, ln & 15, ln >> 4);
+    // 16 rows a step: their weights for both head blocks, and this wave's columns of them
+    vec8_t<E> pf[4][2], vv[4][DT];
+    auto load = [&](int k) {
+      if (k >= 4) return;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(theirs + 256 * j + 4 * lane);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[4 * j + i] = s[8 * KD + 4 * j + i] + x[i];
-      }
-      if (uniform(t * 64 + 64 > len)) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (t * 64 + 32 * u + 16 * KD + (j & 3) + 8 * (j >> 2) + 4 * h >= len) v[j] = -INFINITY;
-      }
-      float mx = v[0];
-#pragma unroll
-      for (int j = 1; j < 8; ++j) mx = fmaxf(mx, v[j]);
-      mx = fmaxf(mx, swap_halves(mx)) * p.scale_log2;
-      const float m_own = hb ? m_run[1] : m_run[0];
-      const bool grown = __any(mx > m_own + kRescaleLog2);
-      // weights over the reference so far: right unless a head outgrew it by 2^kRescaleLog2, which is seen at the barrier
-      auto weigh = [&](float m) {
-        const float m_use = m == -INFINITY ? 0.f : m;
-        float e[8], sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          e[j] = fast_exp2(v[j] * p.scale_log2 - m_use);
-          sum += e[j];
-        }
-        *reinterpret_cast<vec8_t<E>*>(theirs + 4 * lane) =
-            (vec8_t<E>){(E)e[0], (E)e[1], (E)e[2], (E)e[3], (E)e[4], (E)e[5], (E)e[6], (E)e[7]};
-        return sum;
-      };
-      float sum = weigh(m_own);
-      if (h == 0) theirs[256 + r] = mx;
-      if (lane == 0) theirs[288] = grown ? 1.f : 0.f;
-      __syncthreads();
-      if (__any(xbuf[lane & 7][288] != 0.f)) {
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          float m_new = m_run[x];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) m_new = fmaxf(m_new, xbuf[4 * (k >> 1) + 2 * x + (k & 1)][256 + r]);
-          const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run[x] - m_new);
-          m_run[x] = m_new;
-          if (x == hb) l_run *= alpha;
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) o[x][dt] *= alpha;
-        }
-        sum = weigh(hb ? m_run[1] : m_run[0]);
-        __syncthreads();
-      }
-      l_run += sum;
-      // weights of 64 rows: fragment (u, s2, head block x) lies with wave (u, x, 1 - s2)
-      vec8_t<E> pf[2][4];
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          pf[x][k] = *reinterpret_cast<const vec8_t<E>*>(xbuf[2 * (2 * (1 - (k & 1)) + x) + (k >> 1)] + 4 * lane);
-      TrFrag<128, 1> vf = vf0;
-      pin(vf.at);
+      for (int x = 0; x < 2; ++x) pf[k][x] = lds_read_b128(&pbuf[k][x][8 * ln]);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         const int col = w * DT + dt;  // 32-column tile of the latent vector
         TrFrag<128, 1> vc = vf;
         vc.at ^= (col % 4) << 5;
-        const E* vi = img + col / 4 * TI;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const vec8_t<E> a = vc.read(vi, 0, 16 * k);
-          o[0][dt] = mfma32(a, pf[0][k], o[0][dt]);
-          if (blocks > 1) o[1][dt] = mfma32(a, pf[1][k], o[1][dt]);
-        }
+        vv[k][dt] = vc.read(img + col / 4 * TI, 0, 16 * k);
       }
+    };
+#pragma unroll
+    for (int k = 0; k < 1; ++k) load(k);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      load(k + 1);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) o[x][dt] = mfma32(vv[k][dt], pf[k][x], o[x][dt]);
+      __builtin_amdgcn_sched_barrier(0);  // no more fragments in flight than there are registers
     }
-  };
-  if (w < 4) walk(std::integral_constant<int, 0>{});
-  else walk(std::integral_constant<int, 1>{});
+  }
 
-  const float l_pair = l_run + swap_halves(l_run);
-  __syncthreads();  // the last tile's weights have been read
-  if (h == 0) xbuf[w][r] = l_pair;
+  __syncthreads();
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    float l = l_run[x] + swap_quarters(l_run[x]);
+    l += swap_halves(l);
+    if (g4 == 0) smax[kq][32 * hb + 16 * x + i16] = l;
+  }
   __syncthreads();
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
@@ -255,8 +271,8 @@ __global__ __launch_bounds__(kLatentThreads, 2) void latent_attend_kernel(Latent
     if (hd >= p.H) continue;
     const int64_t slot = ((int64_t)b * p.H + hd) * p.ns + part;
     if (w == 0 && h == 0) {
-      p.ml[2 * slot] = m_run[x];
-      p.ml[2 * slot + 1] = (xbuf[2 * x][r] + xbuf[2 * x + 1][r]) + (xbuf[4 + 2 * x][r] + xbuf[4 + 2 * x + 1][r]);
+      p.ml[2 * slot] = m_o[x];
+      p.ml[2 * slot + 1] = (smax[0][32 * x + r] + smax[1][32 * x + r]) + (smax[2][32 * x + r] + smax[3][32 * x + r]);
     }
     if (t0 < t1) store_rows_f32<DT>(p.o + slot * R + w * DT * 32, o[x], 1.f, h);  // an empty part is not read
   }
