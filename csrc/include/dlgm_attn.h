@@ -266,4 +266,17 @@ __device__ __forceinline__ void store_rows_f32(float* row, const f32x16* acc, fl
     }
 }
 
+// acc = f0 acc + f1 row, rows as store_rows_f32 wrote them
+template <int DT>
+__device__ __forceinline__ void add_rows_f32(const float* row, f32x16* acc, float f0, float f1, int h) {
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(row + dt * 32 + 8 * g + 4 * h);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[dt][4 * g + j] = acc[dt][4 * g + j] * f0 + v[j] * f1;
+    }
+}
+
 }  // namespace dlgm

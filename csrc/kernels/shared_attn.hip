@@ -62,15 +62,18 @@ struct SharedArgs {
   __device__ __forceinline__ int plen(int g) const { return plens ? clamp_len(plens[g], P) : P; }
 };
 
-// ---- forward: one workgroup per (b, q head, 128 queries)
-template <typename E, int DA, int DB, int DV, bool PRE>
-__global__ __launch_bounds__(kThreads, 2) void shared_fwd_kernel(SharedArgs<E> p) {
+// ---- forward: one workgroup per (b, q head, 128 queries). SPLIT 2: two waves to 32 queries, each taking every other tile,
+// joined at the end -- for grids that leave a CU no second workgroup, whose only wave a SIMD then waits out every latency
+// (3 x 777 ragged, 8 heads (128, 64, 128), 168 workgroups: 25.4 us with one, 22.3 with two; dQ 35.6 and 32.8).
+template <typename E, int DA, int DB, int DV, bool PRE, int SPLIT>
+__global__ __launch_bounds__(kThreads * SPLIT, 2) void shared_fwd_kernel(SharedArgs<E> p) {
   constexpr int KA = DA / 16, KB = DB / 16, KK = KA + KB, DT = DV / 32;
   constexpr int TA = kBKV * DA, TB = kBKV * DB, TV = kBKV * DV, SLOT = TA + TB + TV;
   constexpr int DBX = DB ? DB : 32;
-  __shared__ __attribute__((aligned(16))) E smem[2 * SLOT];
+  __shared__ __attribute__((aligned(16))) E smem[2 * SPLIT * SLOT];
 
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int w = wid & 3, half = SPLIT > 1 ? wid >> 2 : 0;  // this wave's rows, and which tiles it takes
   const int r = lane & 31, h = lane >> 5, i16 = lane & 15, g4 = lane >> 4;
   const int nqt = (p.S + kBQ - 1) / kBQ, group = p.Hq / p.Hkv;
   // workgroups of one (prefix group, kv head) read the same keys: they follow each other on one XCD, longest first
@@ -96,8 +99,10 @@ __global__ __launch_bounds__(kThreads, 2) void shared_fwd_kernel(SharedArgs<E> p
   const RowTile<E, DA, kBKV, 0> ka(w, lane);
   const RowTile<E, DBX, kBKV, 0> kr(w, lane);
   const RowTile<E, DV, kBKV, 2> va(w, lane);
-  auto stage = [&](int buf, int t) {
-    E* img = smem + buf * SLOT;
+  auto stage = [&](int buf, int step) {
+    const int t = step * SPLIT + half;
+    if (SPLIT > 1 && t >= nt) return;
+    E* img = smem + (buf * SPLIT + half) * SLOT;
     if (PRE && t < np) {
       const int row0 = t * kBKV;
       ka.issue(img, pkb + (int64_t)row0 * p.pk_ss, p.pk_ss, plen - row0, w);
@@ -124,16 +129,19 @@ __global__ __launch_bounds__(kThreads, 2) void shared_fwd_kernel(SharedArgs<E> p
   TrFrag<DV, 2> vf(h, i16, g4);
 
   // unrolled by two: the LDS buffer is a compile-time constant in each copy (immediate ds_read offsets)
-  auto tile = [&](auto bufc, int t) {
+  const int steps = (nt + SPLIT - 1) / SPLIT;
+  auto tile = [&](auto bufc, int step) {
     constexpr int buf = decltype(bufc)::value;
     vm_drain();       // this tile's DMA has landed (this wave's pieces) ...
     __syncthreads();  // ... and every wave's; the other buffer's readers are done
-    if (t + 1 < nt) stage(buf ^ 1, t + 1);
+    if (step + 1 < steps) stage(buf ^ 1, step + 1);
+    const int t = step * SPLIT + half;
+    if (SPLIT > 1 && t >= nt) return;
     const bool pre = PRE && t < np;
     const int kv0 = pre ? t * kBKV : (t - np) * kBKV, end = pre ? plen : len;
     const bool causal = p.causal && !pre;
     if (causal && kv0 > q0w + 31) return;  // whole tile above this wave's diagonal
-    const E* ki = smem + buf * SLOT;
+    const E* ki = smem + (buf * SPLIT + half) * SLOT;
     const E* vi = ki + TA + TB;
     f32x16 s[2] = {(f32x16)(0.f), (f32x16)(0.f)};
 #pragma unroll
@@ -187,28 +195,47 @@ __global__ __launch_bounds__(kThreads, 2) void shared_fwd_kernel(SharedArgs<E> p
         for (int s2 = 0; s2 < 2; ++s2)
           o[dt] = mfma32(vf.read(vi, dt, 32 * u + 16 * s2), pf[u][s2], o[dt]);
   };
-  for (int t = 0; t < nt; t += 2) {
+  for (int t = 0; t < steps; t += 2) {
     tile(std::integral_constant<int, 0>{}, t);
-    if (t + 1 < nt) tile(std::integral_constant<int, 1>{}, t + 1);
+    if (t + 1 < steps) tile(std::integral_constant<int, 1>{}, t + 1);
   }
 
-  const float l_tot = l_run + swap_halves(l_run);
+  float l_tot = l_run + swap_halves(l_run);
+  if constexpr (SPLIT > 1) {
+    constexpr int LD = DV + 4;
+    static_assert(sizeof(E) * 2 * SPLIT * SLOT >= 4 * kBQ * (LD + 2), "the second half's rows fit the tiles' space");
+    float* row = reinterpret_cast<float*>(smem) + (32 * w + r) * LD;
+    float* ml = reinterpret_cast<float*>(smem) + kBQ * LD + 2 * (32 * w + r);
+    __syncthreads();  // every tile has been read
+    if (half) {
+      store_rows_f32<DT>(row, o, 1.f, h);
+      if (h == 0) ml[0] = m_run, ml[1] = l_tot;
+    }
+    __syncthreads();
+    if (half) return;
+    const float m = fmaxf(m_run, ml[0]);
+    const float f0 = l_tot == 0.f ? 0.f : fast_exp2(m_run - m), f1 = ml[1] == 0.f ? 0.f : fast_exp2(ml[0] - m);
+    l_tot = l_tot * f0 + ml[1] * f1;
+    m_run = m;
+    add_rows_f32<DT>(row, o, f0, f1, h);
+  }
   const bool some = qcol < len && l_tot != 0.f;  // a padded query row: zeros and -inf
   store_rows_bf16<DT>(p.out + (((int64_t)b * p.S + qcol) * p.Hq + hq) * DV, o, some ? 1.f / l_tot : 0.f, h, qcol < p.S);
   if (qcol < p.S && h == 0)
     p.lse[((int64_t)b * p.Hq + hq) * p.S + qcol] = some ? (m_run + log2f(l_tot)) * kLn2 : -INFINITY;
 }
 
-// ---- dQ: one workgroup per (b, q head, 128 queries), the forward's walk. It holds dO in registers, so it also forms
+// ---- dQ: one workgroup per (b, q head, 128 queries), the forward's walk and split. It holds dO in registers, so it also forms
 // delta and writes the [-delta, -lse/scale] rows the dK/dV pass starts its accumulators from (padded rows: 0, 0).
-template <typename E, int DA, int DB, int DV, bool PRE>
-__global__ __launch_bounds__(kThreads, 2) void shared_bwd_dq_kernel(SharedArgs<E> p) {
+template <typename E, int DA, int DB, int DV, bool PRE, int SPLIT>
+__global__ __launch_bounds__(kThreads * SPLIT, 2) void shared_bwd_dq_kernel(SharedArgs<E> p) {
   constexpr int KA = DA / 16, KB = DB / 16, KK = KA + KB, KV = DV / 16, DT = (DA + DB) / 32;
   constexpr int TA = kBKV * DA, TB = kBKV * DB, TV = kBKV * DV, SLOT = TA + TB + TV;
   constexpr int DBX = DB ? DB : 32;
-  __shared__ __attribute__((aligned(16))) E smem[2 * SLOT];
+  __shared__ __attribute__((aligned(16))) E smem[2 * SPLIT * SLOT];
 
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int w = wid & 3, half = SPLIT > 1 ? wid >> 2 : 0;  // this wave's rows, and which tiles it takes
   const int r = lane & 31, h = lane >> 5, i16 = lane & 15, g4 = lane >> 4;
   const int nqt = (p.S + kBQ - 1) / kBQ, group = p.Hq / p.Hkv;
   const int work = xcd_remap(blockIdx.x, gridDim.x);
@@ -233,8 +260,10 @@ __global__ __launch_bounds__(kThreads, 2) void shared_bwd_dq_kernel(SharedArgs<E
   const RowTile<E, DA, kBKV, 1> ka(w, lane);
   const RowTile<E, DBX, kBKV, 1> kr(w, lane);
   const RowTile<E, DV, kBKV, 0> va(w, lane);
-  auto stage = [&](int buf, int t) {
-    E* img = smem + buf * SLOT;
+  auto stage = [&](int buf, int step) {
+    const int t = step * SPLIT + half;
+    if (SPLIT > 1 && t >= nt) return;
+    E* img = smem + (buf * SPLIT + half) * SLOT;
     if (PRE && t < np) {
       const int row0 = t * kBKV;
       ka.issue(img, pkb + (int64_t)row0 * p.pk_ss, p.pk_ss, plen - row0, w);
@@ -270,7 +299,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_bwd_dq_kernel(SharedArgs<E
       lse2 = p.lse[rowc] * kLog2e;
     }
     nd = -(acc + swap_halves(acc));
-    if (qcol < p.S && h == 0) {
+    if (qcol < p.S && h == 0 && half == 0) {
       p.rows[rowc] = nd;
       p.rows[(int64_t)p.B * p.Hq * p.S + rowc] = in ? p.lse[rowc] * p.neg_inv_scale : 0.f;
     }
@@ -285,16 +314,19 @@ __global__ __launch_bounds__(kThreads, 2) void shared_bwd_dq_kernel(SharedArgs<E
   TrFrag<DA, 1> kt(h, i16, g4);
   TrFrag<DBX, 1> krt(h, i16, g4);
 
-  auto tile = [&](auto bufc, int t) {
+  const int steps = (nt + SPLIT - 1) / SPLIT;
+  auto tile = [&](auto bufc, int step) {
     constexpr int buf = decltype(bufc)::value;
     vm_drain();
     __syncthreads();
-    if (t + 1 < nt) stage(buf ^ 1, t + 1);
+    if (step + 1 < steps) stage(buf ^ 1, step + 1);
+    const int t = step * SPLIT + half;
+    if (SPLIT > 1 && t >= nt) return;
     const bool pre = PRE && t < np;
     const int kv0 = pre ? t * kBKV : (t - np) * kBKV, end = pre ? plen : len;
     const bool causal = p.causal && !pre;
     if (causal && kv0 > q0w + 31) return;
-    const E* ki = smem + buf * SLOT;
+    const E* ki = smem + (buf * SPLIT + half) * SLOT;
     const E* vi = ki + TA + TB;
     const bool need_mask = uniform((causal && kv0 + kBKV - 1 > q0w) || kv0 + kBKV > end);
 #pragma unroll
@@ -328,9 +360,19 @@ __global__ __launch_bounds__(kThreads, 2) void shared_bwd_dq_kernel(SharedArgs<E
         }
     }
   };
-  for (int t = 0; t < nt; t += 2) {
+  for (int t = 0; t < steps; t += 2) {
     tile(std::integral_constant<int, 0>{}, t);
-    if (t + 1 < nt) tile(std::integral_constant<int, 1>{}, t + 1);
+    if (t + 1 < steps) tile(std::integral_constant<int, 1>{}, t + 1);
+  }
+  if constexpr (SPLIT > 1) {
+    constexpr int LD = DA + DB + 4;
+    static_assert(sizeof(E) * 2 * SPLIT * SLOT >= 4 * kBQ * LD, "the second half's rows fit the tiles' space");
+    float* row = reinterpret_cast<float*>(smem) + (32 * w + r) * LD;
+    __syncthreads();  // every tile has been read
+    if (half) store_rows_f32<DT>(row, dqt, 1.f, h);
+    __syncthreads();
+    if (half) return;
+    add_rows_f32<DT>(row, dqt, 1.f, 1.f, h);
   }
   store_rows_bf16<DT>(p.dq + (((int64_t)b * p.S + qcol) * p.Hq + hq) * (DA + DB), dqt, p.scale, h, qcol < p.S);
 }
@@ -712,6 +754,9 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(SumArgs<E> a) {
   }
 }
 
+// forward and dQ: two waves to 32 queries where the grid leaves every CU at most one workgroup
+bool split_tiles(int64_t blocks) { return blocks <= 256; }
+
 // q, kv, k_rope of latent attention: (nope, value) head dims, refused where no kernel is built for them
 std::pair<int, int> check_latent(const at::Tensor& q, const at::Tensor& kv, const at::Tensor& k_rope, const char* op) {
   check_rows(q, q, op, "q", 4);
@@ -796,8 +841,13 @@ std::tuple<at::Tensor, at::Tensor> dlgm_latent_attn_fwd(const at::Tensor& q, con
   DLGM_DISPATCH_16(q.scalar_type(), E, {
     auto p = latent_args<E>(q, kv, k_rope, dn, lp, softmax_scale, causal);
     p.out = ptr<E>(out), p.lse = lse.data_ptr<float>();
-    if (dn == 128) shared_fwd_kernel<E, 128, 64, 128, false><<<blocks, kThreads, 0, stream>>>(p);
-    else shared_fwd_kernel<E, 64, 32, 64, false><<<blocks, kThreads, 0, stream>>>(p);
+    auto run = [&](auto sc) {
+      constexpr int SP = decltype(sc)::value;
+      if (dn == 128) shared_fwd_kernel<E, 128, 64, 128, false, SP><<<blocks, kThreads * SP, 0, stream>>>(p);
+      else shared_fwd_kernel<E, 64, 32, 64, false, SP><<<blocks, kThreads * SP, 0, stream>>>(p);
+    };
+    if (split_tiles(blocks)) run(std::integral_constant<int, 2>{});
+    else run(std::integral_constant<int, 1>{});
   });
   DLGM_CHECK_HIP(hipGetLastError());
   return {out, lse};
@@ -839,11 +889,16 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> dlgm_latent_attn_bwd(const at::Te
     p.dq = ptr<E>(dq), p.dk = ptr<E>(dkv), p.dv = ptr<E>(dkv) + dn;
     p.dk_ss = p.dv_ss = H * (dn + dv), p.dk_sh = p.dv_sh = dn + dv;
     p.dkr_part = dkr_part.data_ptr<float>();
+    auto dq_pass = [&](auto sc) {
+      constexpr int SP = decltype(sc)::value;
+      if (dn == 128) shared_bwd_dq_kernel<E, 128, 64, 128, false, SP><<<blocks, kThreads * SP, 0, stream>>>(p);
+      else shared_bwd_dq_kernel<E, 64, 32, 64, false, SP><<<blocks, kThreads * SP, 0, stream>>>(p);
+    };
+    if (split_tiles(blocks)) dq_pass(std::integral_constant<int, 2>{});
+    else dq_pass(std::integral_constant<int, 1>{});
     if (dn == 128) {
-      shared_bwd_dq_kernel<E, 128, 64, 128, false><<<blocks, kThreads, 0, stream>>>(p);
       latent_bwd_dkdv_kernel<E, 128, 64, 128><<<blocks, kKvThreads, 0, stream>>>(p);
     } else {
-      shared_bwd_dq_kernel<E, 64, 32, 64, false><<<blocks, kThreads, 0, stream>>>(p);
       latent_bwd_dkdv_kernel<E, 64, 32, 64><<<blocks, kKvThreads, 0, stream>>>(p);
     }
     SumArgs<E> a{};
@@ -875,8 +930,13 @@ std::tuple<at::Tensor, at::Tensor> dlgm_prefix_attn_fwd(const at::Tensor& q, con
   DLGM_DISPATCH_16(q.scalar_type(), E, {
     auto p = prefix_args<E>(q, k, v, prefix_k, prefix_v, lp, pp, softmax_scale, causal);
     p.out = ptr<E>(out), p.lse = lse.data_ptr<float>();
-    if (q.size(3) == 128) shared_fwd_kernel<E, 128, 0, 128, true><<<blocks, kThreads, 0, stream>>>(p);
-    else shared_fwd_kernel<E, 64, 0, 64, true><<<blocks, kThreads, 0, stream>>>(p);
+    auto run = [&](auto sc) {
+      constexpr int SP = decltype(sc)::value;
+      if (q.size(3) == 128) shared_fwd_kernel<E, 128, 0, 128, true, SP><<<blocks, kThreads * SP, 0, stream>>>(p);
+      else shared_fwd_kernel<E, 64, 0, 64, true, SP><<<blocks, kThreads * SP, 0, stream>>>(p);
+    };
+    if (split_tiles(blocks)) run(std::integral_constant<int, 2>{});
+    else run(std::integral_constant<int, 1>{});
   });
   DLGM_CHECK_HIP(hipGetLastError());
   return {out, lse};
@@ -945,7 +1005,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> dlgm_pref
     if (gp * nsplit > 1) p.dpk_part = dpk_part.data_ptr<float>(), p.dpv_part = dpv_part.data_ptr<float>();
     auto run = [&](auto dc) {
       constexpr int DD = decltype(dc)::value;
-      shared_bwd_dq_kernel<E, DD, 0, DD, true><<<q_blocks, kThreads, 0, stream>>>(p);
+      if (split_tiles(q_blocks)) shared_bwd_dq_kernel<E, DD, 0, DD, true, 2><<<q_blocks, 2 * kThreads, 0, stream>>>(p);
+      else shared_bwd_dq_kernel<E, DD, 0, DD, true, 1><<<q_blocks, kThreads, 0, stream>>>(p);
       if (hp == 2) prefix_bwd_dkdv_kernel<E, DD, 2><<<k_blocks, kThreads, 0, stream>>>(p);
       else prefix_bwd_dkdv_kernel<E, DD, 1><<<k_blocks, kThreads, 0, stream>>>(p);
     };

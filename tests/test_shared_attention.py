@@ -93,7 +93,13 @@ def spoil(t, alive, value=float("nan")):
     return t
 
 
-def check_latent(dev, dt, layout, B, S, H, causal=True, lens=None, strided=False, scale=None):
+def ramp(t, dim, lo, hi):
+    """Keys that grow along the sequence, so that a running maximum is raised again and again."""
+    f = torch.linspace(lo, hi, t.shape[dim], device=t.device).view([-1 if i == dim else 1 for i in range(t.dim())])
+    return t.copy_((t.float() * f).to(t.dtype))
+
+
+def check_latent(dev, dt, layout, B, S, H, causal=True, lens=None, strided=False, scale=None, grow=False):
     dn, dr, dv = layout
     g = torch.Generator().manual_seed(B * 1000 + S)
     if strided:  # views of wider rows, the rope key inside the latent projection's row
@@ -104,6 +110,8 @@ def check_latent(dev, dt, layout, B, S, H, causal=True, lens=None, strided=False
     else:
         q, kv = rnd(g, B, S, H, dn + dr, dt=dt, dev=dev), rnd(g, B, S, H, dn + dv, dt=dt, dev=dev)
         kr, do = rnd(g, B, S, dr, dt=dt, dev=dev), rnd(g, B, S, H, dv, dt=dt, dev=dev)
+    if grow:
+        ramp(kv[..., :dn], 1, 0.1, 8), ramp(kr, 1, 0.1, 8)
     alive = live(lens, B, S, dev)
     for t in (q, kv, kr, do):
         spoil(t, alive)
@@ -127,7 +135,7 @@ def check_latent(dev, dt, layout, B, S, H, causal=True, lens=None, strided=False
         assert not t[~alive].any(), "rows behind a length are zeros"
 
 
-def check_prefix(dev, dt, D, G, n, P, S, Hq, Hkv, causal=True, lens=None, plens=None, strided=False):
+def check_prefix(dev, dt, D, G, n, P, S, Hq, Hkv, causal=True, lens=None, plens=None, strided=False, grow=False):
     B, rep = G * n, Hq // Hkv
     g = torch.Generator().manual_seed(P * 1000 + S)
     if strided:  # q, k, v as parts of one packed row; the prefix cut from a longer one
@@ -138,6 +146,8 @@ def check_prefix(dev, dt, D, G, n, P, S, Hq, Hkv, causal=True, lens=None, plens=
         q, k, v = (rnd(g, B, S, h, D, dt=dt, dev=dev) for h in (Hq, Hkv, Hkv))
         pk, pv = (rnd(g, G, P, Hkv, D, dt=dt, dev=dev) for _ in range(2))
     do = rnd(g, B, S, Hq, D, dt=dt, dev=dev)
+    if grow:
+        ramp(pk, 1, 0.1, 4), ramp(k, 1, 4, 8)
     alive, palive = live(lens, B, S, dev), live(plens, G, P, dev)
     for t in (q, k, v, do):
         spoil(t, alive)
@@ -165,9 +175,11 @@ def check_prefix(dev, dt, D, G, n, P, S, Hq, Hkv, causal=True, lens=None, plens=
         assert not t[~a].any(), "rows behind a length are zeros"
 
 
-def check_latent_decode(dev, dt, layout, r, B, H, L, lens, strided=False):
+def check_latent_decode(dev, dt, layout, r, B, H, L, lens, strided=False, grow=False):
     """Four roundings (absorbed query, weights, latent output, result), each off by at most u of what it rounds: 4 u in
-    the 2-norm of a head's output."""
+    the 2-norm of a head's output. `grow`: queries of 3 times the size; the absorbed query's rounding, r independent ones of at
+    most u, moves a score by u / sqrt(3) times its own size, some 3 in the mean, and a weight and its sum by that factor each:
+    3.5 u more, 8 u in all."""
     dn, dr, dv = layout
     g = torch.Generator().manual_seed(B * 1000 + L)
     w = rnd(g, H * (dn + dv), r, dt=dt, dev=dev, std=r ** -0.5)
@@ -176,6 +188,8 @@ def check_latent_decode(dev, dt, layout, r, B, H, L, lens, strided=False):
         cache = rnd(g, L, B, r + dr + 32, dt=dt, dev=dev).transpose(0, 1)[..., :r + dr]
     else:
         q, cache = rnd(g, B, H, dn + dr, dt=dt, dev=dev), rnd(g, B, L, r + dr, dt=dt, dev=dev)
+    if grow:
+        q.mul_(3), ramp(cache, 1, 0.05, 1)
     alive = live(lens, B, L, dev)
     spoil(cache, alive)
     out = ops.latent_attention_decode(q, cache, torch.tensor(lens, dtype=torch.int32, device=dev), w)
@@ -186,11 +200,11 @@ def check_latent_decode(dev, dt, layout, r, B, H, L, lens, strided=False):
                     (dn + dr) ** -0.5, dt)["out"][0].squeeze(2)
     u = torch.finfo(dt).eps / 2 if dt != torch.float32 else 2.0 ** -20
     err = (out.double() - want).norm(dim=-1)
-    assert (err <= 4 * u * want.norm(dim=-1)).all(), float((err / want.norm(dim=-1).clamp_min(1e-30)).max())
+    assert (err <= (8 if grow else 4) * u * want.norm(dim=-1)).all(), float((err / want.norm(dim=-1).clamp_min(1e-30)).max())
     assert not out[~alive[:, 0]].any()
 
 
-def check_prefix_decode(dev, dt, D, G, n, P, L, Hq, Hkv, lens, plens=None, strided=False):
+def check_prefix_decode(dev, dt, D, G, n, P, L, Hq, Hkv, lens, plens=None, strided=False, grow=False):
     B, rep = G * n, Hq // Hkv
     g = torch.Generator().manual_seed(P * 1000 + L)
     q = rnd(g, Hq, B, D, dt=dt, dev=dev).transpose(0, 1) if strided else rnd(g, B, Hq, D, dt=dt, dev=dev)
@@ -200,6 +214,8 @@ def check_prefix_decode(dev, dt, D, G, n, P, L, Hq, Hkv, lens, plens=None, strid
     else:
         k, v = (rnd(g, B, L, Hkv, D, dt=dt, dev=dev) for _ in range(2))
         pk, pv = (rnd(g, G, P, Hkv, D, dt=dt, dev=dev) for _ in range(2))
+    if grow:
+        ramp(pk, 1, 0.1, 4), ramp(k, 1, 4, 8)
     alive, palive = live(lens, B, L, dev), live(plens, G, P, dev)
     for t in (k, v):
         spoil(t, alive)
@@ -293,6 +309,8 @@ BF, FP = torch.bfloat16, torch.float16
     (FP, HALF, 4, 200, 2, True, [1, 200, 31, 97], False),
     (BF, HALF, 2, 65, 1, False, [65, 33], True),
     (FP, HALF, 1, 640, 9, True, None, False),
+    (BF, WIDE, 3, 257, 30, True, [257, 100, 0], False),  # more workgroups than CUs: one wave to 32 queries
+    (FP, HALF, 2, 130, 70, False, None, True),
 ])
 def test_latent_kernels(dt, layout, B, S, H, causal, lens, strided):
     check_latent(GPU, dt, layout, B, S, H, causal, lens, strided)
@@ -309,6 +327,8 @@ def test_latent_kernels(dt, layout, B, S, H, causal, lens, strided):
     (FP, 64, 1, 5, 64, 129, 12, 12, True, [129, 64, 0, 1, 100], None, False),
     (BF, 64, 1, 2, 513, 17, 6, 1, False, None, [0], False),
     (FP, 64, 1, 8, 1000, 3, 2, 2, True, None, None, False),
+    (BF, 128, 2, 4, 200, 140, 24, 4, True, [140, 1, 139, 0, 64, 65, 128, 140], [200, 7], False),  # more workgroups than CUs
+    (FP, 64, 1, 9, 70, 60, 30, 10, False, None, None, False),
 ])
 def test_prefix_kernels(dt, D, G, n, P, S, Hq, Hkv, causal, lens, plens, strided):
     check_prefix(GPU, dt, D, G, n, P, S, Hq, Hkv, causal, lens, plens, strided)
@@ -324,6 +344,7 @@ def test_prefix_kernels(dt, D, G, n, P, S, Hq, Hkv, causal, lens, plens, strided
     (BF, HALF, 512, 2, 20, 513, [500, 513], False),
     (FP, HALF, 256, 1, 130, 4100, [4100], False),
     (BF, HALF, 256, 40, 3, 5, [i % 6 for i in range(40)], False),
+    (BF, WIDE, 512, 40, 70, 1000, [1000 - 25 * i for i in range(40)], False),  # several tiles to a workgroup
 ])
 def test_latent_decode_kernel(dt, layout, r, B, H, L, lens, strided):
     check_latent_decode(GPU, dt, layout, r, B, H, L, lens, strided)
@@ -342,6 +363,20 @@ def test_latent_decode_kernel(dt, layout, r, B, H, L, lens, strided):
 ])
 def test_prefix_decode_kernel(dt, D, G, n, P, L, Hq, Hkv, lens, plens, strided):
     check_prefix_decode(GPU, dt, D, G, n, P, L, Hq, Hkv, lens, plens, strided)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [BF, FP])
+def test_growing_scores(dt):
+    """Running maxima that are raised all along the keys (the rescaling branches of every kernel)."""
+    check_latent(GPU, dt, WIDE, 1, 400, 2, False, grow=True)
+    check_latent(GPU, dt, HALF, 1, 400, 2, True, grow=True)
+    check_prefix(GPU, dt, 128, 1, 2, 300, 100, 4, 2, grow=True)
+    check_prefix(GPU, dt, 64, 1, 2, 300, 100, 2, 2, False, grow=True)
+    check_latent_decode(GPU, dt, WIDE, 512, 40, 66, 900, [900] * 40, grow=True)
+    check_latent_decode(GPU, dt, HALF, 256, 40, 3, 900, [900] * 40, grow=True)
+    check_prefix_decode(GPU, dt, 128, 1, 40, 3000, 100, 4, 1, [100] * 40, grow=True)
+    check_prefix_decode(GPU, dt, 64, 2, 3, 3000, 100, 4, 2, [100] * 6, grow=True)
 
 
 def _train_inputs(seed, dev=GPU, dt=BF):
