@@ -4,6 +4,7 @@
 // token layer: 239 us a training pass that way). The forward and backward operators go through the dispatcher, so
 // whatever observes operators (the stream audit) sees them with their arguments.
 #include <torch/all.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/DeviceGuard.h>
@@ -42,11 +43,16 @@ void check_latent(const at::Tensor& q, const at::Tensor& c, const at::Tensor& k_
               ": c and k_rope must have q's batch and length, c the columns of w_kv");
   TORCH_CHECK(H > 0 && w_kv.size(0) % H == 0 && w_kv.size(0) / H > q.size(3) - k_rope.size(2), op,
               ": w_kv must have nope + value rows per head");
-  TORCH_CHECK(r % 8 == 0, op, ": the latent size must be a multiple of 8, got ", r);
+  TORCH_CHECK(r > 0 && r % 8 == 0, op, ": the latent size must be a positive multiple of 8, got ", r);
 }
 
-// c, w_kv as GEMM operands: rows of r values
-at::Tensor flat(const at::Tensor& t, int64_t cols) { return t.reshape({-1, cols}).contiguous(); }
+// c, w_kv as GEMM operands: rows of r values, copied only where the library's vector loads could not read them in place
+at::Tensor flat(const at::Tensor& t, int64_t cols) {
+  const auto x = t.reshape({-1, cols});
+  const bool aligned = reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+  if (aligned && x.stride(1) == 1 && x.stride(0) % 8 == 0 && x.stride(0) >= cols) return x;
+  return x.clone(at::MemoryFormat::Contiguous);
+}
 
 // kv = c w_kv^T by one dense GEMM, then the attention
 std::tuple<at::Tensor, at::Tensor, at::Tensor> latent_attention_fwd(const at::Tensor& q, const at::Tensor& c,
@@ -57,7 +63,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> latent_attention_fwd(const at::Te
   const c10::DeviceGuard guard(q.device());
   const int64_t r = w_kv.size(1), n = w_kv.size(0);
   auto kv = at::empty({q.size(0), q.size(1), q.size(2), n / q.size(2)}, q.options());
-  if (kv.numel() > 0) dlgm_gemm_lt(kv.view({-1, n}), flat(c, r), w_kv.contiguous().t(), 0.0, -1);
+  if (kv.numel() > 0) dlgm_gemm_lt(kv.view({-1, n}), flat(c, r), flat(w_kv, r).t(), 0.0, -1);
   auto [out, lse] = dlgm_latent_attn_fwd(q, kv, k_rope, softmax_scale, causal, lens);
   return {out, lse, kv};
 }
@@ -74,7 +80,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> latent_attention_bwd(
   auto dc = at::empty(c.sizes(), c.options()), dw = at::empty(w_kv.sizes(), w_kv.options());
   if (dkv.numel() == 0) return {dq, dc.zero_(), dkr, dw.zero_()};
   const auto d2 = dkv.view({-1, n});
-  dlgm_gemm_lt(dc.view({-1, r}), d2, w_kv.contiguous(), 0.0, -1);
+  dlgm_gemm_lt(dc.view({-1, r}), d2, flat(w_kv, r), 0.0, -1);
   // dw = dkv^T c reduces over the rows of both. The library runs it at some 1.0 PFLOP/s as it lies and at 1.27 with c's
   // columns contiguous; transposing c costs its bytes at 4.5 TB/s and a launch, so large products transpose (8192 tokens,
   // 32 x 256 columns, r 512: 102 -> 82 us)
@@ -90,6 +96,22 @@ auto op(const char* name) {
   return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
 }
 
+// Gradients recorded for a second differentiation (create_graph) with regard to the inputs raise an error there: no kernel
+// has a second derivative. `all`: as many entries as the forward has arguments, the gradients first.
+variable_list once(variable_list grads, const Variable& dout, const variable_list& saved, size_t all) {
+  const size_t n = grads.size();
+  if (at::GradMode::is_enabled()) {
+    grads.push_back(dout);
+    grads.insert(grads.end(), saved.begin(), saved.begin() + n);  // the inputs, in their order
+    const auto inputs = static_cast<int64_t>(grads.size());
+    grads = (*std::make_shared<torch::autograd::DelayedError>(
+        "a gradient of latent_attention or prefix_attention cannot be differentiated again", inputs))(std::move(grads));
+    grads.resize(n);
+  }
+  grads.resize(all);
+  return grads;
+}
+
 struct LatentAttention : public torch::autograd::Function<LatentAttention> {
   static at::Tensor forward(AutogradContext* ctx, const Variable& q, const Variable& c, const Variable& k_rope,
                             const Variable& w_kv, double softmax_scale, bool causal, const OptTensor& lens) {
@@ -103,11 +125,12 @@ struct LatentAttention : public torch::autograd::Function<LatentAttention> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list dout) {
     const auto s = ctx->get_saved_variables();
+    at::AutoDispatchBelowADInplaceOrView below;
     static auto bwd = op<decltype(latent_attention_bwd)>("dlgm::latent_attention_bwd");
     auto [dq, dc, dkr, dw] =
         bwd.call(dout[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6], ctx->saved_data["scale"].toDouble(),
                  ctx->saved_data["causal"].toBool(), s[7].defined() ? OptTensor(s[7]) : c10::nullopt);
-    return {dq, dc, dkr, dw, Variable(), Variable(), Variable()};
+    return once({dq, dc, dkr, dw}, dout[0], s, 7);
   }
 };
 
@@ -133,12 +156,13 @@ struct PrefixAttention : public torch::autograd::Function<PrefixAttention> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list dout) {
     const auto s = ctx->get_saved_variables();
+    at::AutoDispatchBelowADInplaceOrView below;
     static auto bwd = op<PrefixBwd>("dlgm::prefix_attn_bwd");
     auto [dq, dk, dv, dpk, dpv] =
         bwd.call(dout[0].contiguous(), s[0], s[1], s[2], s[3], s[4], s[5], s[6], ctx->saved_data["scale"].toDouble(),
                  ctx->saved_data["causal"].toBool(), s[7].defined() ? OptTensor(s[7]) : c10::nullopt,
                  s[8].defined() ? OptTensor(s[8]) : c10::nullopt);
-    return {dq, dk, dv, dpk, dpv, Variable(), Variable(), Variable(), Variable()};
+    return once({dq, dk, dv, dpk, dpv}, dout[0], s, 9);
   }
 };
 

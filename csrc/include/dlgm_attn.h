@@ -124,11 +124,6 @@ __device__ __forceinline__ void glds4(const void* src, void* lds) {
   __builtin_amdgcn_global_load_lds((gptr_t)src, (lptr_t)lds, 4, 0, 0);
 }
 __device__ __forceinline__ void vm_drain() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-// all but this wave's N youngest vector-memory operations are done
-template <int N>
-__device__ __forceinline__ void vm_wait() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
 
 // One LDS-DMA piece through a buffer descriptor (buffer_load_dwordx4 ... lds): `base` and `nbytes`
 // are wave-uniform (the descriptor lives in SGPRs, reads at or past nbytes return zero), `voff`
@@ -148,7 +143,7 @@ __device__ __forceinline__ int xcd_remap(int id, int total) {
   return (id % 8) * (total / 8) + id / 8;
 }
 
-// LDS-DMA whose arrival only the kernel's own waits (vm_drain, vm_wait) follow. After the builtin the compiler waits for
+// LDS-DMA whose arrival only the kernel's own waits (vm_drain) follow. After the builtin the compiler waits for
 // every load in flight before the next LDS read that it cannot tell apart from the landing place (any transposed read, any
 // buffer chosen at run time): the next tile then loads before, not during, the work on this one -- measured 266 against
 // 166 us of work and 156 us of loads alone in the latent attend kernel. An LDS-DMA has no destination register, so nothing
@@ -194,7 +189,7 @@ struct RowTile {
     col = 16 * (SWZ == 2 ? swz_tr<D>(row, phys) : SWZ == 1 ? swz_dual<D>(row, phys) : swz_row<D>(row, phys));
   }
   __device__ __forceinline__ void issue(E* img, const E* base, int64_t stride, int valid, int wave) const {
-    if (NP < NW) wave %= NP;  // fewer pieces than waves: some load one twice, so every wave issues PPW loads
+    if (NP < NW) wave %= NP;  // fewer pieces than waves: some load one twice, which costs less than a branch
     const int bytes = valid > 0 ? (int)((int64_t)(min(valid, ROWS) - 1) * stride * 2) + D * 2 : 0;
     const uint32_t step = (uint32_t)(stride * 2);
     uint32_t off = (uint32_t)row * step + col;

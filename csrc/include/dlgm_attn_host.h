@@ -3,12 +3,11 @@
 #pragma once
 
 #include <torch/all.h>
-#include <cmath>
 #include "dlgm_common.h"
 
 namespace dlgm {
 
-constexpr int kThreads = 256;  // of every shared-key attention kernel
+constexpr int kThreads = 256;  // of a workgroup, where a kernel does not say otherwise
 
 inline void check_rows(const at::Tensor& t, const at::Tensor& like, const char* op, const char* name, int dim) {
   TORCH_CHECK(t.is_cuda() && t.device() == like.device(), op, ": ", name, " must be on the device of q");
@@ -25,7 +24,7 @@ inline void check_rows(const at::Tensor& t, const at::Tensor& like, const char* 
 }
 
 inline const int* check_lens(const c10::optional<at::Tensor>& lens, const at::Tensor& like, int64_t n, const char* op,
-                      const char* name) {
+                             const char* name) {
   if (!lens.has_value() || !lens->defined()) return nullptr;
   TORCH_CHECK(lens->device() == like.device() && lens->scalar_type() == at::kInt && lens->is_contiguous() &&
                   lens->dim() == 1 && lens->numel() == n,
@@ -33,8 +32,9 @@ inline const int* check_lens(const c10::optional<at::Tensor>& lens, const at::Te
   return lens->data_ptr<int>();
 }
 
+// the backward starts its scores from -lse / scale, in fp32
 inline void check_scale(double s, const char* op) {
-  TORCH_CHECK(std::isfinite(s) && s > 0, op, ": softmax_scale must be positive");
+  TORCH_CHECK(s >= 1e-20 && s <= 1e20, op, ": softmax_scale must lie between 1e-20 and 1e20, got ", s);
 }
 
 // HIP needs gridDim.x * blockDim.x below 2^32

@@ -14,7 +14,7 @@
 //             rows -- fp32 partials summed in a fixed order, no atomics: bits do not depend on scheduling.
 // P and dS are rounded to the 16-bit type before their products: they are matrix-instruction operands.
 //
-// Structure: 4 waves of 32 query rows (forward, dQ) or 32 keys (dK/dV), tiles by LDS-DMA one tile ahead, XOR-swizzled
+// Structure: waves of 32 query rows (forward, dQ) or 32 keys (dK/dV), tiles by LDS-DMA one tile ahead, XOR-swizzled
 // images, transposed operands by ds_read_b64_tr_b16. A tile's descriptor covers exactly its valid rows, so rows past a
 // length read as zero whatever memory holds there (a score is masked besides), and a tile's base is a 64-bit address:
 // no offset of a long sequence passes 32 bits.
@@ -225,8 +225,8 @@ __global__ __launch_bounds__(kThreads * SPLIT, 2) void shared_fwd_kernel(SharedA
     p.lse[((int64_t)b * p.Hq + hq) * p.S + qcol] = some ? (m_run + log2f(l_tot)) * kLn2 : -INFINITY;
 }
 
-// ---- dQ: one workgroup per (b, q head, 128 queries), the forward's walk and split. It holds dO in registers, so it also forms
-// delta and writes the [-delta, -lse/scale] rows the dK/dV pass starts its accumulators from (padded rows: 0, 0).
+// ---- dQ: one workgroup per (b, q head, 128 queries), the forward's walk and split. It holds dO in registers, so it also
+// forms delta and writes the [-delta, -lse/scale] rows the dK/dV pass starts its accumulators from (padded rows: 0, 0).
 template <typename E, int DA, int DB, int DV, bool PRE, int SPLIT>
 __global__ __launch_bounds__(kThreads * SPLIT, 2) void shared_bwd_dq_kernel(SharedArgs<E> p) {
   constexpr int KA = DA / 16, KB = DB / 16, KK = KA + KB, KV = DV / 16, DT = (DA + DB) / 32;
@@ -377,9 +377,9 @@ __global__ __launch_bounds__(kThreads * SPLIT, 2) void shared_bwd_dq_kernel(Shar
   store_rows_bf16<DT>(p.dq + (((int64_t)b * p.S + qcol) * p.Hq + hq) * (DA + DB), dqt, p.scale, h, qcol < p.S);
 }
 
-// ---- dK / dV over a shared prefix: one workgroup per (128 keys, HP q heads of one kv head, a range of sequences). Keys of a sequence are
-// seen by that sequence alone; keys of a prefix by the n sequences of its group, walked one after the other into the
-// same accumulators (cut into nsplit parts where the prefix alone gives too few workgroups).
+// ---- dK / dV over a shared prefix: one workgroup per (128 keys, HP q heads of one kv head, a range of sequences). Keys
+// of a sequence are seen by that sequence alone; keys of a prefix by the n sequences of its group, walked one after the
+// other into the same accumulators (cut into nsplit parts where the prefix alone gives too few workgroups).
 // A wave of 32 keys keeps K and the gradients in registers and V in LDS: two waves a SIMD. (The split of the latent kernel
 // below, two waves to 32 keys, measured 1622 us here against 1306 at 8 x 1024 queries over 4096 + 1024 keys, 32/8 heads.)
 template <typename E, int D, int HP>
@@ -734,7 +734,7 @@ __global__ __launch_bounds__(kKvThreads, 2) void latent_bwd_dkdv_kernel(SharedAr
   }
 }
 
-// Sum of the fp32 parts in a fixed order -> 16 bits. Up to four tensors in one launch (grid.y).
+// Sum of the fp32 parts in a fixed order -> 16 bits: dk_rope, or up to four tensors of a prefix backward (grid.y)
 template <typename E>
 struct SumArgs {
   const float* part[4];
@@ -768,7 +768,7 @@ std::pair<int, int> check_latent(const at::Tensor& q, const at::Tensor& kv, cons
   const int64_t dr = k_rope.size(2), dn = q.size(3) - dr, dv = kv.size(3) - dn;
   TORCH_CHECK((dn == 128 && dr == 64 && dv == 128) || (dn == 64 && dr == 32 && dv == 64), op,
               ": head dims (nope, rope, value) must be (128, 64, 128) or (64, 32, 64), got (", dn, ", ", dr, ", ", dv, ")");
-  TORCH_CHECK(S < INT32_MAX / 2 && B * H < INT32_MAX, op, ": too many rows");
+  TORCH_CHECK(S < INT32_MAX / 4 && B * H < INT32_MAX, op, ": too many rows");
   return {(int)dn, (int)dv};
 }
 
@@ -802,7 +802,7 @@ void check_prefix(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
               ": prefix_k and prefix_v must be [G, P, Hkv, D]");
   TORCH_CHECK(Hkv > 0 && Hq % Hkv == 0, op, ": q heads must be a multiple of the kv heads");
   TORCH_CHECK(G > 0 && B % G == 0, op, ": the batch must hold equally many sequences of each prefix");
-  TORCH_CHECK(S < INT32_MAX / 2 && pk.size(1) < INT32_MAX / 2 && B * Hq < INT32_MAX, op, ": too many rows");
+  TORCH_CHECK(S < INT32_MAX / 4 && pk.size(1) < INT32_MAX / 2 && B * Hq < INT32_MAX, op, ": too many rows");
 }
 
 template <typename E>
@@ -880,7 +880,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> dlgm_latent_attn_bwd(const at::Te
   const auto f32 = q.options().dtype(at::kFloat);
   auto rows = at::empty({2, B, H, S}, f32);
   auto dkr_part = at::empty({H, B, S, dr}, f32);
-  const int64_t blocks = check_blocks(B * H * ((S + kBQ - 1) / kBQ), op);
+  const int64_t blocks = check_blocks(2 * B * H * ((S + kBQ - 1) / kBQ), op) / 2;  // dK/dV: of 512 threads
   auto stream = c10::hip::getCurrentHIPStream();
   DLGM_DISPATCH_16(q.scalar_type(), E, {
     auto p = latent_args<E>(q, kv, k_rope, dn, lp, softmax_scale, causal);

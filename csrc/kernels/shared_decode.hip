@@ -67,7 +67,8 @@ __global__ __launch_bounds__(kThreads) void latent_absorb_kernel(LatentArgs<E> p
     for (int s = 0; s < DN / 16; ++s) {
       vec8_t<E> f = (vec8_t<E>)((E)0.f);
       if (b < p.B)  // the k order of the transposed read: rows 16 s + 4 h .. +3, then the same + 8
-        f = cat(*reinterpret_cast<const vec4_t<E>*>(q + 16 * s + 4 * h), *reinterpret_cast<const vec4_t<E>*>(q + 16 * s + 8 + 4 * h));
+        f = cat(*reinterpret_cast<const vec4_t<E>*>(q + 16 * s + 4 * h),
+                *reinterpret_cast<const vec4_t<E>*>(q + 16 * s + 8 + 4 * h));
       acc = mfma32(a[s], f, acc);
     }
     const f32x16 acc1[1] = {acc};
@@ -244,8 +245,7 @@ __global__ __launch_bounds__(kLatentThreads, 2) void latent_attend_kernel(Latent
         vv[k][dt] = vc.read(img + col / 4 * TI, 0, 16 * k);
       }
     };
-#pragma unroll
-    for (int k = 0; k < 1; ++k) load(k);
+    load(0);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       load(k + 1);
@@ -688,7 +688,7 @@ at::Tensor dlgm_prefix_attn_decode(const at::Tensor& q, const at::Tensor& k, con
   const int64_t rep = Hq / Hkv, n = B / G, psteps = (P + kStep - 1) / kStep, osteps = (L + kStep - 1) / kStep;
   const int prw = row_waves(n * rep), orw = row_waves(rep);
   const int64_t prb = (n * rep + 32 * prw - 1) / (32 * prw), orb = (rep + 32 * orw - 1) / (32 * orw);
-  // both kinds of workgroup get about the same number of steps, 1024 workgroups in all, of which 512 run at a time
+  // both kinds of workgroup get about the same number of steps, 512 workgroups in all: two a CU, all at once
   const int64_t pitems = G * Hkv * prb, oitems = B * Hkv * orb;
   const int64_t per = std::max<int64_t>(1, (pitems * psteps + oitems * osteps + 511) / 512);
   const int64_t np = P ? parts_of(psteps, 1, (psteps + per - 1) / per) : 0;
@@ -696,7 +696,7 @@ at::Tensor dlgm_prefix_attn_decode(const at::Tensor& q, const at::Tensor& k, con
   if (np + no == 0) return out.zero_();
   auto o = at::empty({B, Hq, np + no, D}, q.options().dtype(at::kFloat));
   auto ml = at::empty({B, Hq, np + no, 2}, q.options().dtype(at::kFloat));
-  const int64_t blocks = check_blocks(pitems * np + oitems * no, op);
+  const int64_t blocks = check_blocks(pitems * np + oitems * no, op), rows = check_blocks(B * Hq, op);
   auto stream = c10::hip::getCurrentHIPStream();
   DLGM_DISPATCH_16(q.scalar_type(), E, {
     PrefixArgs<E> p{};
@@ -712,10 +712,10 @@ at::Tensor dlgm_prefix_attn_decode(const at::Tensor& q, const at::Tensor& k, con
     p.scale_log2 = softmax_scale * kLog2e;
     if (D == 128) {
       prefix_attend_kernel<E, 128><<<blocks, kThreads, 0, stream>>>(p);
-      prefix_join_kernel<E, 128><<<B * Hq, kThreads, 0, stream>>>(p);
+      prefix_join_kernel<E, 128><<<rows, kThreads, 0, stream>>>(p);
     } else {
       prefix_attend_kernel<E, 64><<<blocks, kThreads, 0, stream>>>(p);
-      prefix_join_kernel<E, 64><<<B * Hq, kThreads, 0, stream>>>(p);
+      prefix_join_kernel<E, 64><<<rows, kThreads, 0, stream>>>(p);
     }
   });
   DLGM_CHECK_HIP(hipGetLastError());

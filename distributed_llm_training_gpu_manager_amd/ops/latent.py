@@ -96,6 +96,16 @@ def latent_attn_bwd(dout: torch.Tensor, q: torch.Tensor, kv: torch.Tensor, k_rop
     return back(torch.matmul(ds, kf)), back(dkv), dk[..., dn:].sum(1).to(q.dtype)
 
 
+def once(grads: Tuple[torch.Tensor, ...], inputs: Tuple[torch.Tensor, ...]) -> Tuple[torch.Tensor, ...]:
+    """Gradients recorded for a second differentiation (create_graph) with regard to ``inputs`` raise an error there: no
+    kernel has one."""
+    if not torch.is_grad_enabled():
+        return grads
+    args = [g.detach() for g in grads] + list(inputs)
+    msg = "a gradient of latent_attention or prefix_attention cannot be differentiated again"
+    return tuple(torch._C._functions.DelayedError(msg, len(args))(*args)[:len(grads)])
+
+
 class LatentAttentionFunction(torch.autograd.Function):
     """Expanded form: kv = c w_kv^T, attention, and in the backward dc = dkv w_kv, dw_kv = dkv^T c. The latent vectors and
     the packed kv rows are saved (kv again costs a GEMM, its rows H (nope + value) values a token)."""
@@ -114,9 +124,9 @@ class LatentAttentionFunction(torch.autograd.Function):
         q, c, k_rope, w_kv, kv, out, lse, lens = ctx.saved_tensors
         dq, dkv, dkr = latent_attn_bwd(dout.contiguous(), q, kv, k_rope, out, lse, ctx.scale, ctx.causal, lens)
         dkv2, c2 = dkv.view(-1, w_kv.shape[0]), c.reshape(-1, c.shape[-1])
-        dc = mm(dkv2, w_kv).view(c.shape) if ctx.needs_input_grad[1] else None
-        dw = grad_mm(torch.empty_like(w_kv), dkv2.t(), c2, False) if ctx.needs_input_grad[3] else None
-        return dq, dc, dkr, dw, None, None, None
+        with torch.no_grad():
+            dc, dw = mm(dkv2, w_kv).view(c.shape), grad_mm(torch.empty_like(w_kv), dkv2.t(), c2, False)
+        return (*once((dq, dc, dkr, dw), (dout, q, c, k_rope, w_kv)), None, None, None)
 
 
 def latent_attention(q: torch.Tensor, c: torch.Tensor, k_rope: torch.Tensor, w_kv: torch.Tensor,

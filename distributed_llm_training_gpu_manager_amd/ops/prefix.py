@@ -20,7 +20,7 @@ from typing import Optional, Tuple
 import torch
 
 from .._native import hip_ops, use_native
-from .latent import Lens, live_rows, softmax_lse
+from .latent import Lens, live_rows, once, softmax_lse
 
 
 def _scale(q: torch.Tensor, softmax_scale: Optional[float]) -> float:
@@ -111,7 +111,7 @@ class PrefixAttentionFunction(torch.autograd.Function):
     def backward(ctx, dout):
         q, k, v, pk, pv, out, lse, lens, plens = ctx.saved_tensors
         g = prefix_attn_bwd(dout.contiguous(), q, k, v, pk, pv, out, lse, ctx.scale, ctx.causal, lens, plens)
-        return (*g, None, None, None, None)
+        return (*once(g, (dout, q, k, v, pk, pv)), None, None, None, None)
 
 
 def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor,

@@ -260,6 +260,22 @@ def test_gradients_match_differences(lens):
                                     (x(2, 4, 4, 3), x(2, 4, 2, 3), x(2, 4, 2, 3), x(1, 3, 2, 3), x(1, 3, 2, 3)))
 
 
+@pytest.mark.parametrize("dev", [CPU, pytest.param(GPU, marks=pytest.mark.gpu)])
+def test_a_second_differentiation_is_refused(dev):
+    """Gradients may be recorded (create_graph), for losses that use others of them; differentiating these raises."""
+    q, kv, kr = (t.requires_grad_(True) for t in _latent_args(dev))
+    g = torch.Generator().manual_seed(4)
+    c, w = (rnd(g, *s, dt=q.dtype, dev=dev).requires_grad_(True) for s in ((2, 8, 16), (2 * 128, 16)))
+    k, pk = (rnd(g, *s, dt=q.dtype, dev=dev).requires_grad_(True) for s in ((2, 8, 2, 64), (1, 5, 2, 64)))
+    for out, x in ((ops.latent_attention(q, c, kr, w), (q, c, kr, w)), (ops.prefix_attention(q[..., :64], k, k, pk, pk), (k, pk))):
+        plain = torch.autograd.grad(out.sum(), x, retain_graph=True)
+        recorded = torch.autograd.grad(out.sum(), x, create_graph=True)
+        assert all(torch.equal(a, b.detach()) for a, b in zip(plain, recorded))
+        for r in recorded:
+            with pytest.raises(RuntimeError, match="differentiated again"):
+                torch.autograd.grad(r.sum(), x, allow_unused=True, retain_graph=True)
+
+
 def test_absorbed_and_expanded_agree():
     """The last token of the expanded form is the absorbed form over the cache of all tokens."""
     g = torch.Generator().manual_seed(1)
@@ -511,6 +527,99 @@ def test_runs_on_the_current_stream():
 
 
 @pytest.mark.gpu
+def test_two_calls_at_once():
+    """Calls on two streams do not share a workspace: each gives what it gives alone."""
+    args = [_train_inputs(i) for i in (10, 11)]
+    lens = torch.tensor([150, 99], dtype=torch.int32, device=GPU)
+
+    def whole(q, c, kr, w, do):
+        leaves = [t.clone().requires_grad_(True) for t in (q, c, kr, w)]
+        out = ops.latent_attention(*leaves, lens=lens)
+        return (out.detach(), *torch.autograd.grad(out, leaves, do), ops.latent_attention_decode(q[:, 3], torch.cat([c, kr], -1), lens, w))
+
+    alone = [whole(*a) for a in args]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        got = []
+        for s, a in zip(streams, args):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(whole(*a))
+        torch.cuda.synchronize()
+        for x, y in zip(got, alone):
+            assert all(torch.equal(i, j) for i, j in zip(x, y))
+
+
+@pytest.mark.gpu
+def test_differentiable_calls_are_captured():
+    """Forward and gradients of both differentiable entry points in one graph, replayed on new values."""
+    q, c, kr, w, do = (t.requires_grad_(i < 4) for i, t in enumerate(_train_inputs(12)))
+    g = torch.Generator().manual_seed(13)
+    x = [rnd(g, *s, dt=BF, dev=GPU).requires_grad_(True) for s in ((2, 40, 4, 64), (2, 40, 2, 64), (2, 40, 2, 64), (1, 90, 2, 64), (1, 90, 2, 64))]
+    xdo = rnd(g, 2, 40, 4, 64, dt=BF, dev=GPU)
+
+    def both():
+        a, b = ops.latent_attention(q, c, kr, w), ops.prefix_attention(*x)
+        return (a.detach(), b.detach(), *torch.autograd.grad(a, (q, c, kr, w), do), *torch.autograd.grad(b, x, xdo))
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        both()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=s):
+            outs = both()
+    torch.cuda.current_stream().wait_stream(s)
+    for i in range(3):
+        with torch.no_grad():
+            for t in (q, c, w, x[0], x[3]):
+                t.mul_(0.8 + 0.2 * i)
+        gr.replay()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):  # the same library workspace as the captured calls
+            want = both()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want)), i
+
+
+@pytest.mark.gpu
+def test_odd_arguments():
+    """Lengths outside the tensors' count as their ends; views that a GEMM cannot read in place; no gradient to record."""
+    q, c, kr, w, do = _train_inputs(14)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=GPU)  # noqa: E731
+    full = ops.latent_attention(q, c, kr, w, lens=i32(150, 0))
+    assert torch.equal(full, ops.latent_attention(q, c, kr, w, lens=i32(1 << 30, -5)))
+    cache = torch.cat([c, kr], -1)
+    assert torch.equal(ops.latent_attention_decode(q[:, 0], cache, i32(1 << 30, -5), w), ops.latent_attention_decode(q[:, 0], cache, i32(150, 0), w))
+    pk = rnd(torch.Generator().manual_seed(15), 1, 30, 2, 64, dt=BF, dev=GPU)
+    k, pq = pk[:, :9].repeat(2, 1, 1, 1), torch.ones(2, 4, 64, dtype=BF, device=GPU)
+    a = ops.prefix_attention_decode(pq, k, k, i32(99, -1), pk, pk, i32(77))
+    assert torch.equal(a, ops.prefix_attention_decode(pq, k, k, i32(9, 0), pk, pk))
+    # rows of a wider tensor, and contiguous weights at an odd address
+    wide = torch.zeros(2, 150, c.shape[-1] + 8, dtype=BF, device=GPU)
+    wide[..., :c.shape[-1]] = c
+    odd = torch.zeros(w.numel() + 1, dtype=BF, device=GPU)[1:].view_as(w).copy_(w)
+    leaves = [t.clone().requires_grad_(True) for t in (q, c, kr, w)]
+    views = [leaves[0].detach(), wide[..., :c.shape[-1]], kr, odd]
+    views = [v.detach().requires_grad_(True) for v in views]
+    res = []
+    for x in (leaves, views):
+        out = ops.latent_attention(*x)
+        res.append((out.detach(), *torch.autograd.grad(out.sum(), x)))  # an expanded dO
+    u = torch.finfo(BF).eps / 2
+    for x, y in zip(*res):  # another GEMM may be picked for other strides: each result within its 6 u of the exact one
+        assert float((x.double() - y.double()).norm()) <= 12 * u * float(x.double().norm())
+    with torch.no_grad():
+        a = ops.latent_attention(q, c, kr, w)
+    with torch.inference_mode():
+        b = ops.latent_attention(q, c, kr, w)
+        ops.prefix_attention(pq.unsqueeze(1), k[:, :1], k[:, :1], pk, pk)
+    assert torch.equal(a, b) and not a.requires_grad
+    assert torch.equal(a, ops.latent_attention(*leaves))
+
+
+@pytest.mark.gpu
 def test_rows_beyond_32_bit_offsets():
     """Row strides and cache lengths whose byte offsets pass 32 bits."""
     dn, dr, dv = HALF
@@ -561,6 +670,10 @@ def test_kernels_refuse_what_they_cannot_do():
         lambda: ops.latent_attn_fwd(q, kv, kr, lens=i32(8)),
         lambda: ops.latent_attn_fwd(q, kv, kr, lens=i32(8, 8).cpu()),
         lambda: ops.latent_attn_fwd(q, kv, kr, softmax_scale=0.0),
+        lambda: ops.latent_attn_fwd(q, kv, kr, softmax_scale=1e-30),
+        lambda: ops.latent_attn_fwd(q, kv, kr, softmax_scale=1e30),
+        lambda: ops.latent_attention(q, kr[..., :0], kr, kr.new_zeros(256, 0)),
+        lambda: ops.latent_attention(q, kr[..., :12], kr, kr.new_zeros(256, 12)),
         lambda: ops.latent_attn_fwd(q, kv, kr, softmax_scale=float("nan")),
         lambda: ops.latent_attn_fwd(q.transpose(2, 3), kv, kr),
         lambda: ops.latent_attn_fwd(torch.zeros(2, 8, 2, 97, dtype=BF, device=GPU)[..., 1:], kv, kr),
