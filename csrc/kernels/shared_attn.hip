@@ -76,11 +76,13 @@ __global__ __launch_bounds__(kThreads * SPLIT, 2) void shared_fwd_kernel(SharedA
   const int w = wid & 3, half = SPLIT > 1 ? wid >> 2 : 0;  // this wave's rows, and which tiles it takes
   const int r = lane & 31, h = lane >> 5, i16 = lane & 15, g4 = lane >> 4;
   const int nqt = (p.S + kBQ - 1) / kBQ, group = p.Hq / p.Hkv;
-  // workgroups of one (prefix group, kv head) read the same keys: they follow each other on one XCD, longest first
-  const int work = xcd_remap(blockIdx.x, gridDim.x);
-  const int per_kv = p.n * group * nqt;
-  const int bk = work / per_kv, rem = work - bk * per_kv;
-  const int qt = nqt - 1 - rem / (p.n * group), idx = rem % (p.n * group);
+  // the longest first, over all heads. Workgroups go to the XCDs in turn, so those of one (prefix group, kv head), which
+  // read the same keys at about the same time, share an XCD where these are a multiple of 8. (Head by head on one XCD each,
+  // two long ones met on every CU: 450 and 416 us at 2 x 4096 tokens, 32 heads (128, 64, 128), 82 and 71 at 2 x 2048, 16;
+  // no gain from the XCD alone at 5 x 1300, 20 heads: 103 and 91.)
+  const int per_kv = p.n * group, nbk = p.B / p.n * p.Hkv;
+  const int bk = blockIdx.x % nbk, rem = blockIdx.x / nbk;
+  const int qt = nqt - 1 - rem / per_kv, idx = rem % per_kv;
   const int grp = bk / p.Hkv, hk = bk % p.Hkv, hq = hk * group + idx % group, b = grp * p.n + idx / group;
 
   const int len = p.len(b);
@@ -238,10 +240,9 @@ __global__ __launch_bounds__(kThreads * SPLIT, 2) void shared_bwd_dq_kernel(Shar
   const int w = wid & 3, half = SPLIT > 1 ? wid >> 2 : 0;  // this wave's rows, and which tiles it takes
   const int r = lane & 31, h = lane >> 5, i16 = lane & 15, g4 = lane >> 4;
   const int nqt = (p.S + kBQ - 1) / kBQ, group = p.Hq / p.Hkv;
-  const int work = xcd_remap(blockIdx.x, gridDim.x);
-  const int per_kv = p.n * group * nqt;
-  const int bk = work / per_kv, rem = work - bk * per_kv;
-  const int qt = nqt - 1 - rem / (p.n * group), idx = rem % (p.n * group);
+  const int per_kv = p.n * group, nbk = p.B / p.n * p.Hkv;
+  const int bk = blockIdx.x % nbk, rem = blockIdx.x / nbk;
+  const int qt = nqt - 1 - rem / per_kv, idx = rem % per_kv;
   const int grp = bk / p.Hkv, hk = bk % p.Hkv, hq = hk * group + idx % group, b = grp * p.n + idx / group;
 
   const int len = p.len(b);
@@ -407,13 +408,11 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_bwd_dkdv_kernel(SharedArgs
     b0 = grp * p.n + p.n * part / p.nsplit;
     b1 = grp * p.n + p.n * (part + 1) / p.nsplit;
   } else {
-    const int id = blockIdx.x - p.prefix_blocks;
-    const int work = xcd_remap(id, gridDim.x - p.prefix_blocks);
-    const int nkt = (p.S + kBQ - 1) / kBQ;
-    k0 = work % nkt * kBQ;  // ascending: most queries first under the causal mask
-    const int x = work / nkt;
-    hq = x % nhp * HP;
-    b0 = x / nhp;
+    // the first keys first, over all heads (2 x 2048 tokens, 32/8 heads, the whole backward: 354 us head by head, 314 so)
+    const int id = blockIdx.x - p.prefix_blocks, nbh = p.B * nhp;
+    k0 = id / nbh * kBQ;
+    hq = id % nbh % nhp * HP;
+    b0 = id % nbh / nhp;
     b1 = b0 + 1;
   }
   const int hk = hq / group, hh = hq % group, grp = b0 / p.n;
@@ -568,9 +567,9 @@ __global__ __launch_bounds__(kKvThreads, 2) void latent_bwd_dkdv_kernel(SharedAr
 
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 31, h = lane >> 5, i16 = lane & 15, g4 = lane >> 4;
-  const int nkt = (p.S + kBQ - 1) / kBQ;
-  const int work = xcd_remap(blockIdx.x, gridDim.x);  // blocks of one (b, head) share their Q / dO stream
-  const int k0 = work % nkt * kBQ, hd = work / nkt % p.Hq, b = work / nkt / p.Hq;  // ascending: most queries first
+  // the first keys, which most queries see, first, over all heads; blocks of one head share its Q / dO stream (3 x 1111
+  // tokens, 16 heads, the whole backward: 157 us head by head, 134 so)
+  const int bh = blockIdx.x % (p.B * p.Hq), k0 = blockIdx.x / (p.B * p.Hq) * kBQ, hd = bh % p.Hq, b = bh / p.Hq;
   const int len = p.len(b);
   const int kg = w & 3, kw0 = k0 + 32 * kg, key = kw0 + r;
   const RowTile<E, DA, kBQ2, 1, 8> qa(w, lane);
@@ -754,8 +753,11 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(SumArgs<E> a) {
   }
 }
 
-// forward and dQ: two waves to 32 queries where the grid leaves every CU at most one workgroup
-bool split_tiles(int64_t blocks) { return blocks <= 256; }
+// forward and dQ: two waves to 32 queries where the grid leaves every CU at most one workgroup; and where it leaves two to
+// latent attention over long sequences, whose first and last tiles differ so much that the second 256 workgroups are better
+// handed out as the first end (1 x 4096 tokens, 16 heads: forward 133 and 116 us, backward 421 and 394; but 4 x 1024: 41
+// and 43, 162 and 165)
+bool split_tiles(int64_t blocks, int64_t tiles = 0) { return blocks <= 256 || (blocks <= 512 && tiles >= 16); }
 
 // q, kv, k_rope of latent attention: (nope, value) head dims, refused where no kernel is built for them
 std::pair<int, int> check_latent(const at::Tensor& q, const at::Tensor& kv, const at::Tensor& k_rope, const char* op) {
@@ -846,7 +848,7 @@ std::tuple<at::Tensor, at::Tensor> dlgm_latent_attn_fwd(const at::Tensor& q, con
       if (dn == 128) shared_fwd_kernel<E, 128, 64, 128, false, SP><<<blocks, kThreads * SP, 0, stream>>>(p);
       else shared_fwd_kernel<E, 64, 32, 64, false, SP><<<blocks, kThreads * SP, 0, stream>>>(p);
     };
-    if (split_tiles(blocks)) run(std::integral_constant<int, 2>{});
+    if (split_tiles(blocks, (p.S + kBQ - 1) / kBQ)) run(std::integral_constant<int, 2>{});
     else run(std::integral_constant<int, 1>{});
   });
   DLGM_CHECK_HIP(hipGetLastError());
@@ -894,7 +896,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> dlgm_latent_attn_bwd(const at::Te
       if (dn == 128) shared_bwd_dq_kernel<E, 128, 64, 128, false, SP><<<blocks, kThreads * SP, 0, stream>>>(p);
       else shared_bwd_dq_kernel<E, 64, 32, 64, false, SP><<<blocks, kThreads * SP, 0, stream>>>(p);
     };
-    if (split_tiles(blocks)) dq_pass(std::integral_constant<int, 2>{});
+    if (split_tiles(blocks, (p.S + kBQ - 1) / kBQ)) dq_pass(std::integral_constant<int, 2>{});
     else dq_pass(std::integral_constant<int, 1>{});
     if (dn == 128) {
       latent_bwd_dkdv_kernel<E, 128, 64, 128><<<blocks, kKvThreads, 0, stream>>>(p);
