@@ -592,10 +592,19 @@ __global__ __launch_bounds__(kThreads) void prefix_join_kernel(PrefixArgs<E> p) 
   p.out[row * D + c] = (E)(l == 0.f ? 0.f : o / l);  // a row without keys: zeros
 }
 
-// how many parts a length of `steps` steps is cut into so that `items` such lengths give about `want` workgroups
-int64_t parts_of(int64_t steps, int64_t items, int64_t want) {
-  const int64_t most = 64;  // a join reads every part of a row
-  return std::max<int64_t>(1, std::min({steps, most, (want + items - 1) / std::max<int64_t>(1, items)}));
+constexpr int64_t kMostParts = 64;  // a join reads every part of a row
+
+// Latent attend: how many parts `items` lengths of `steps` tiles are cut into. A CU holds one workgroup, so the call takes
+// (rounds of 256 workgroups) x (tiles of a part + what a workgroup's start and end cost, some 6 tiles); the fewest that make
+// that least. (As many as give 256 workgroups or a few more, rounded up, measured 87 us at 5 x 9000 rows, 128 heads, 87 at
+// 40 x 2000, 64 heads, and 178 at 96 x 3000; so 57, 66 and 138.)
+int64_t latent_parts(int64_t steps, int64_t items) {
+  int64_t best = INT64_MAX, ns = 1;
+  for (int64_t k = 1; k <= std::min(kMostParts, steps); ++k) {
+    const int64_t cost = (items * k + 255) / 256 * ((steps + k - 1) / k + 6);
+    if (cost < best) best = cost, ns = k;
+  }
+  return ns;
 }
 
 // waves along the rows: as many as the rows fill (a step's keys are shared by the rest)
@@ -626,7 +635,7 @@ at::Tensor dlgm_latent_attn_decode(const at::Tensor& q, const at::Tensor& cache,
   if (B == 0) return out;
   if (L == 0) return out.zero_();
   const int64_t nhb = (H + 63) / 64;
-  const int64_t ns = parts_of((L + 63) / 64, B * nhb, 256);
+  const int64_t ns = latent_parts((L + 63) / 64, B * nhb);
   auto qa = at::empty({B, H, r}, q.options());
   auto o = at::empty({B, H, ns, r}, q.options().dtype(at::kFloat));
   auto ml = at::empty({B, H, ns, 2}, q.options().dtype(at::kFloat));
@@ -688,11 +697,20 @@ at::Tensor dlgm_prefix_attn_decode(const at::Tensor& q, const at::Tensor& k, con
   const int64_t rep = Hq / Hkv, n = B / G, psteps = (P + kStep - 1) / kStep, osteps = (L + kStep - 1) / kStep;
   const int prw = row_waves(n * rep), orw = row_waves(rep);
   const int64_t prb = (n * rep + 32 * prw - 1) / (32 * prw), orb = (rep + 32 * orw - 1) / (32 * orw);
-  // both kinds of workgroup get about the same number of steps, 512 workgroups in all: two a CU, all at once
+  // both kinds of workgroup get about the same number of steps, 512 workgroups in all: two a CU, all at once. Where rounding
+  // up the parts gives a few more, which would wait for a second round, parts up to half as long again are taken if they
+  // end that (16 x 700 keys over 8000, 32/8 heads: 26.7 and 22.7 us); longer ones cost more than the round (96 x 256 over
+  // 8192, 64/4 heads, where they would be four times as long: 52 and 99).
   const int64_t pitems = G * Hkv * prb, oitems = B * Hkv * orb;
-  const int64_t per = std::max<int64_t>(1, (pitems * psteps + oitems * osteps + 511) / 512);
-  const int64_t np = P ? parts_of(psteps, 1, (psteps + per - 1) / per) : 0;
-  const int64_t no = L ? parts_of(osteps, 1, (osteps + per - 1) / per) : 0;
+  auto parts = [](int64_t steps, int64_t per) { return std::min(kMostParts, (steps + per - 1) / per); };
+  int64_t per = std::max<int64_t>(1, (pitems * psteps + oitems * osteps + 511) / 512);
+  auto fits = [&](int64_t x) { return pitems * parts(psteps, x) + oitems * parts(osteps, x) <= 512; };
+  for (int64_t x = per, most = per + (per + 1) / 2; x <= most; x += 1 + x / 16)
+    if (fits(x)) {
+      per = x;
+      break;
+    }
+  const int64_t np = parts(psteps, per), no = parts(osteps, per);
   if (np + no == 0) return out.zero_();
   auto o = at::empty({B, Hq, np + no, D}, q.options().dtype(at::kFloat));
   auto ml = at::empty({B, Hq, np + no, 2}, q.options().dtype(at::kFloat));
