@@ -607,7 +607,8 @@ int64_t latent_parts(int64_t steps, int64_t items) {
   return ns;
 }
 
-// waves along the rows: as many as the rows fill (a step's keys are shared by the rest)
+// waves along the rows: as many as the rows fill (a step's keys are shared by the rest). 256 rows over 16384 keys: 94 us of
+// attend with 4, 110 with 2, 153 with 1; 16 rows over 8192: the call 22.8, 21.7 and 21.7.
 int row_waves(int64_t rows) { return rows > 64 ? 4 : rows > 32 ? 2 : 1; }
 
 }  // namespace

@@ -361,6 +361,10 @@ def test_prefix_kernels(dt, D, G, n, P, S, Hq, Hkv, causal, lens, plens, strided
     (FP, HALF, 256, 1, 130, 4100, [4100], False),
     (BF, HALF, 256, 40, 3, 5, [i % 6 for i in range(40)], False),
     (BF, WIDE, 512, 40, 70, 1000, [1000 - 25 * i for i in range(40)], False),  # several tiles to a workgroup
+    (BF, HALF, 512, 150, 4, 700, [0 if 20 <= i < 100 else 7 * i % 701 for i in range(150)], False),  # idle slots in between
+    (FP, WIDE, 256, 200, 130, 130, [(37 * i) % 131 for i in range(200)], False),  # several sequences to a workgroup
+    (BF, WIDE, 512, 70, 2, 9000, [9000 if i == 66 else 0 for i in range(70)], False),  # one of many
+    (BF, WIDE, 512, 3, 8, 100, [0, 0, 0], False),
 ])
 def test_latent_decode_kernel(dt, layout, r, B, H, L, lens, strided):
     check_latent_decode(GPU, dt, layout, r, B, H, L, lens, strided)
