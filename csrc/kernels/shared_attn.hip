@@ -405,8 +405,8 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_bwd_dkdv_kernel(SharedArgs
     x /= nhp;
     part = x % p.nsplit;
     const int grp = x / p.nsplit;
-    b0 = grp * p.n + p.n * part / p.nsplit;
-    b1 = grp * p.n + p.n * (part + 1) / p.nsplit;
+    b0 = grp * p.n + (int)((int64_t)p.n * part / p.nsplit);
+    b1 = grp * p.n + (int)((int64_t)p.n * (part + 1) / p.nsplit);
   } else {
     // the first keys first, over all heads (2 x 2048 tokens, 32/8 heads, the whole backward: 354 us head by head, 314 so)
     const int id = blockIdx.x - p.prefix_blocks, nbh = p.B * nhp;

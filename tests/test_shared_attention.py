@@ -659,6 +659,31 @@ def test_rows_beyond_32_bit_offsets():
 
 
 @pytest.mark.gpu
+def test_group_of_millions():
+    """A group whose sequences times the parts they are cut into (1024 for so short a prefix) pass 31 bits. The prefix's
+    value gradient sums over all of them, positive terms: the weights are off by at most u each, the result once more, and
+    an fp32 chain runs over a part's sequences and then over the parts. Scores of sum |q| |k| < 96 are off by at most (D + 8)
+    2^-24 96 / 8, a weight by twice that: 2^-13."""
+    n, D, P, parts = 2_200_000, 64, 3, 1024
+    g = torch.Generator(device=GPU).manual_seed(16)
+    q, k, v, do = (torch.randn(n, 1, 1, D, generator=g, device=GPU).to(BF) for _ in range(4))
+    do = do.abs()
+    pk, pv = (torch.randn(1, P, 1, D, generator=g, device=GPU).to(BF) for _ in range(2))
+    assert n * (parts - 1) > 2 ** 31
+    out, lse = ops.prefix_attn_fwd(q, k, v, pk, pv)
+    dv, dpv = ops.prefix_attn_bwd(do, q, k, v, pk, pv, out, lse)[2::2]
+    q, k, do = (t.view(n, D).double() for t in (q, k, do))
+    p = torch.softmax(torch.cat([q @ pk.view(P, D).double().t(), (q * k).sum(-1, keepdim=True)], 1) * D ** -0.5, -1)
+    assert float((q * k).abs().sum(-1).max()) < 96 and float((q.abs() @ pk.view(P, D).double().abs().t()).max()) < 96
+    u = torch.finfo(BF).eps / 2
+    want = p[:, :P].t() @ do
+    chain = (n / parts + parts) * F32
+    assert ((dpv.view(P, D).double() - want).abs() <= (2 * u + u * u + 2 ** -13 + chain) * want).all()
+    own = p[:, P:] * do
+    assert ((dv.view(n, D).double() - own).abs() <= (2 * u + u * u + 2 ** -13) * own).all()
+
+
+@pytest.mark.gpu
 def test_kernels_refuse_what_they_cannot_do():
     q, kv, kr = _latent_args(GPU)
     i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=GPU)  # noqa: E731
