@@ -54,6 +54,13 @@ at::Tensor flat(const at::Tensor& t, int64_t cols) {
   return x.clone(at::MemoryFormat::Contiguous);
 }
 
+// A gradient as the kernels read it: contiguous from a 16-byte address on. Autograd may hand on a slice of a larger one
+// (out was concatenated behind something), contiguous from any element on.
+at::Tensor rows16(const at::Tensor& t) {
+  const auto x = t.contiguous();
+  return reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 ? x : x.clone();
+}
+
 // kv = c w_kv^T by one dense GEMM, then the attention
 std::tuple<at::Tensor, at::Tensor, at::Tensor> latent_attention_fwd(const at::Tensor& q, const at::Tensor& c,
                                                                     const at::Tensor& k_rope, const at::Tensor& w_kv,
@@ -76,7 +83,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> latent_attention_bwd(
   check_latent(q, c, k_rope, w_kv);
   const c10::DeviceGuard guard(q.device());
   const int64_t r = w_kv.size(1), n = w_kv.size(0);
-  auto [dq, dkv, dkr] = dlgm_latent_attn_bwd(dout.contiguous(), q, kv, k_rope, out, lse, softmax_scale, causal, lens);
+  auto [dq, dkv, dkr] = dlgm_latent_attn_bwd(rows16(dout), q, kv, k_rope, out, lse, softmax_scale, causal, lens);
   auto dc = at::empty(c.sizes(), c.options()), dw = at::empty(w_kv.sizes(), w_kv.options());
   if (dkv.numel() == 0) return {dq, dc.zero_(), dkr, dw.zero_()};
   const auto d2 = dkv.view({-1, n});
@@ -159,7 +166,7 @@ struct PrefixAttention : public torch::autograd::Function<PrefixAttention> {
     at::AutoDispatchBelowADInplaceOrView below;
     static auto bwd = op<PrefixBwd>("dlgm::prefix_attn_bwd");
     auto [dq, dk, dv, dpk, dpv] =
-        bwd.call(dout[0].contiguous(), s[0], s[1], s[2], s[3], s[4], s[5], s[6], ctx->saved_data["scale"].toDouble(),
+        bwd.call(rows16(dout[0]), s[0], s[1], s[2], s[3], s[4], s[5], s[6], ctx->saved_data["scale"].toDouble(),
                  ctx->saved_data["causal"].toBool(), s[7].defined() ? OptTensor(s[7]) : c10::nullopt,
                  s[8].defined() ? OptTensor(s[8]) : c10::nullopt);
     return once({dq, dk, dv, dpk, dpv}, dout[0], s, 9);

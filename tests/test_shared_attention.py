@@ -624,6 +624,21 @@ def test_odd_arguments():
 
 
 @pytest.mark.gpu
+def test_gradients_that_start_anywhere():
+    """The output behind a single element in a concatenation: its gradient is contiguous from an odd address on."""
+    q, c, kr, w, do = _train_inputs(17)
+    g = torch.Generator().manual_seed(18)
+    x = [rnd(g, *s, dt=BF, dev=GPU) for s in ((2, 40, 4, 64), (2, 40, 2, 64), (2, 40, 2, 64), (1, 90, 2, 64), (1, 90, 2, 64))]
+    for fn, args, grad in ((ops.latent_attention, (q, c, kr, w), do), (ops.prefix_attention, x, rnd(g, 2, 40, 4, 64, dt=BF, dev=GPU))):
+        leaves = [t.clone().requires_grad_(True) for t in args]
+        want = torch.autograd.grad(fn(*leaves), leaves, grad)
+        one = torch.zeros(1, dtype=BF, device=GPU, requires_grad=True)
+        whole = torch.cat([one, fn(*leaves).flatten()])
+        got = torch.autograd.grad(whole, leaves, torch.cat([one.detach(), grad.flatten()]))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
 def test_rows_beyond_32_bit_offsets():
     """Row strides and cache lengths whose byte offsets pass 32 bits."""
     dn, dr, dv = HALF
