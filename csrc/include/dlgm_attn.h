@@ -80,9 +80,11 @@ __device__ __forceinline__ float swap_halves(float x) {
 // each 8-column group k) as bf16, scaled. One half-exchange (v_permlane32_swap) per dword of a group
 // pair (k, k+1) leaves lanes h = 0 with columns 8k .. 8k+7 and lanes h = 1 with 8k+8 .. 8k+15: one
 // 16-byte store per pair instead of two 8-byte stores (the tail is store-issue bound). Both lanes of
-// a pair share the row, so the swap runs on all lanes and only the store is guarded by `valid`.
+// a pair share the row, so the swap runs on all lanes and only the store is guarded by `valid`. A row that is not `live`
+// (behind a length) is stored as zeros whatever its accumulators hold: 0 times a NaN or an infinity of a live row is a NaN.
 template <int DT, typename E>
-__device__ __forceinline__ void store_rows_bf16(E* row, const f32x16 (&acc)[DT], float scale, int h, bool valid) {
+__device__ __forceinline__ void store_rows_bf16(E* row, const f32x16 (&acc)[DT], float scale, int h, bool valid,
+                                                bool live = true) {
 #pragma unroll
   for (int k = 0; k < 4 * DT; k += 2) {
     const f32x16& oa = acc[k >> 2];
@@ -95,7 +97,9 @@ __device__ __forceinline__ void store_rows_bf16(E* row, const f32x16 (&acc)[DT],
     uint2 a = __builtin_bit_cast(uint2, va), c = __builtin_bit_cast(uint2, vb);
     const auto sx = __builtin_amdgcn_permlane32_swap(a.x, c.x, false, false);
     const auto sy = __builtin_amdgcn_permlane32_swap(a.y, c.y, false, false);
-    if (valid) *reinterpret_cast<uint4*>(row + 8 * k + 8 * h) = make_uint4(sx[0], sy[0], sx[1], sy[1]);
+    if (valid)
+      *reinterpret_cast<uint4*>(row + 8 * k + 8 * h) =
+          live ? make_uint4(sx[0], sy[0], sx[1], sy[1]) : make_uint4(0, 0, 0, 0);
   }
 }
 
@@ -253,15 +257,15 @@ struct TrFrag {            // columns 32 dt .. +31 of rows row0 + {4 h .. +3, 8 
   }
 };
 
-// fp32 rows of a transposed accumulator: lane (key r, half h) holds columns 8k + 4h .. +3
+// fp32 rows of a transposed accumulator: lane (key r, half h) holds columns 8k + 4h .. +3; zeros where not `live`
 template <int DT>
-__device__ __forceinline__ void store_rows_f32(float* row, const f32x16* acc, float scale, int h) {
+__device__ __forceinline__ void store_rows_f32(float* row, const f32x16* acc, float scale, int h, bool live = true) {
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const f32x4 v = {acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
-      *reinterpret_cast<f32x4*>(row + dt * 32 + 8 * g + 4 * h) = v * scale;
+      *reinterpret_cast<f32x4*>(row + dt * 32 + 8 * g + 4 * h) = live ? v * scale : (f32x4)(0.f);
     }
 }
 

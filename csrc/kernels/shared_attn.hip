@@ -222,7 +222,7 @@ __global__ __launch_bounds__(kThreads * SPLIT, 2) void shared_fwd_kernel(SharedA
     add_rows_f32<DT>(row, o, f0, f1, h);
   }
   const bool some = qcol < len && l_tot != 0.f;  // a padded query row: zeros and -inf
-  store_rows_bf16<DT>(p.out + (((int64_t)b * p.S + qcol) * p.Hq + hq) * DV, o, some ? 1.f / l_tot : 0.f, h, qcol < p.S);
+  store_rows_bf16<DT>(p.out + (((int64_t)b * p.S + qcol) * p.Hq + hq) * DV, o, 1.f / l_tot, h, qcol < p.S, some);
   if (qcol < p.S && h == 0)
     p.lse[((int64_t)b * p.Hq + hq) * p.S + qcol] = some ? (m_run + log2f(l_tot)) * kLn2 : -INFINITY;
 }
@@ -375,7 +375,7 @@ __global__ __launch_bounds__(kThreads * SPLIT, 2) void shared_bwd_dq_kernel(Shar
     if (half) return;
     add_rows_f32<DT>(row, dqt, 1.f, 1.f, h);
   }
-  store_rows_bf16<DT>(p.dq + (((int64_t)b * p.S + qcol) * p.Hq + hq) * (DA + DB), dqt, p.scale, h, qcol < p.S);
+  store_rows_bf16<DT>(p.dq + (((int64_t)b * p.S + qcol) * p.Hq + hq) * (DA + DB), dqt, p.scale, h, qcol < p.S, in);
 }
 
 // ---- dK / dV over a shared prefix: one workgroup per (128 keys, HP q heads of one kv head, a range of sequences). Keys
@@ -515,6 +515,8 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_bwd_dkdv_kernel(SharedArgs
         dk[dt] = mfma32(qt.read(qi, dt, 16 * s2), dsf[s2], dk[dt]);
       }
   };
+  int left = nkeys - key;  // > 0: this key exists; beside the tiles in a vector register, the scalar ones are spilled here
+  pin(left);
   Cursor cur{-1, 0, 0, 0, 0};
   if (k0 < nkeys && seek(cur)) {
     stage(0, cur);
@@ -540,13 +542,13 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_bwd_dkdv_kernel(SharedArgs
   const int slot = (pre ? part * (group / HP) : 0) + hh / HP;
   const int64_t base = (int64_t)(pre ? grp : b0) * rows + key;
   if (nparts == 1) {
-    store_rows_bf16<DT>((pre ? p.dpk : p.dk) + (base * p.Hkv + hk) * D, dk, p.scale, h, key < rows);
-    store_rows_bf16<DT>((pre ? p.dpv : p.dv) + (base * p.Hkv + hk) * D, dv, 1.f, h, key < rows);
+    store_rows_bf16<DT>((pre ? p.dpk : p.dk) + (base * p.Hkv + hk) * D, dk, p.scale, h, key < rows, left > 0);
+    store_rows_bf16<DT>((pre ? p.dpv : p.dv) + (base * p.Hkv + hk) * D, dv, 1.f, h, key < rows, left > 0);
   } else if (key < rows) {
     const int64_t all = (int64_t)(pre ? p.B / p.n : p.B) * rows;  // rows of a part
     const int64_t at = ((slot * all + base) * p.Hkv + hk) * D;
-    store_rows_f32<DT>((pre ? p.dpk_part : p.dk_part) + at, dk, p.scale, h);
-    store_rows_f32<DT>((pre ? p.dpv_part : p.dv_part) + at, dv, 1.f, h);
+    store_rows_f32<DT>((pre ? p.dpk_part : p.dk_part) + at, dk, p.scale, h, left > 0);
+    store_rows_f32<DT>((pre ? p.dpv_part : p.dv_part) + at, dv, 1.f, h, left > 0);
   }
 }
 
@@ -672,7 +674,7 @@ __global__ __launch_bounds__(kKvThreads, 2) void latent_bwd_dkdv_kernel(SharedAr
 #pragma unroll
             for (int x = 0; x < 4; ++x) dv[dt] = mfma32(dt_.template read<E>(smem, dt, 16 * x), pf[x >> 1][x & 1], dv[dt]);
         });
-    store_rows_bf16<DTV>(p.dv + base * p.dv_ss + hd * p.dv_sh, dv, 1.f, h, key < p.S);
+    store_rows_bf16<DTV>(p.dv + base * p.dv_ss + hd * p.dv_sh, dv, 1.f, h, key < p.S, key < len);
   } else {  // dS and dK, one tile behind
     vec8_t<E> vf[KV];  // B operand of dP = dO V^T
     const E* vb = p.v + b * p.v_sb + hd * p.v_sh + (int64_t)key * p.v_ss + 8 * h;
@@ -728,8 +730,10 @@ __global__ __launch_bounds__(kKvThreads, 2) void latent_bwd_dkdv_kernel(SharedAr
           }
         });
     // one head owns its k_nope rows, the rope part is summed over the heads
-    store_rows_bf16<DTA>(p.dk + base * p.dk_ss + hd * p.dk_sh, *reinterpret_cast<f32x16(*)[DTA]>(dk), p.scale, h, key < p.S);
-    if (key < p.S) store_rows_f32<DB / 32>(p.dkr_part + (((int64_t)hd * p.B + b) * p.S + key) * DB, dk + DTA, p.scale, h);
+    store_rows_bf16<DTA>(p.dk + base * p.dk_ss + hd * p.dk_sh, *reinterpret_cast<f32x16(*)[DTA]>(dk), p.scale, h, key < p.S,
+                         key < len);
+    if (key < p.S)
+      store_rows_f32<DB / 32>(p.dkr_part + (((int64_t)hd * p.B + b) * p.S + key) * DB, dk + DTA, p.scale, h, key < len);
   }
 }
 

@@ -53,19 +53,21 @@ def _scale(q: torch.Tensor, softmax_scale: Optional[float]) -> float:
 
 
 def _ref_parts(q, kv, k_rope, scale, causal, lens):
-    """fp32 (or wider) q, k, v, weights and log-sum-exp, head-major; rows past a length are zeros in all of them."""
+    """fp32 (or wider) q, k, v, weights and log-sum-exp, head-major; rows past a length are zeros in all of them. Also the
+    ways there and back ([B, S, H, ...] -> head-major -> [B, S, H, ...] in q's type), both with zeros past a length."""
     B, S, H, _ = q.shape
     dn, dr, _ = _dims(q, kv, k_rope)
     live = live_rows(lens, B, S, q.device)
     wide = torch.promote_types(q.dtype, torch.float32)
     rows = lambda t: torch.where(live[:, :, None, None], t.to(wide), 0.0).permute(0, 2, 1, 3)  # noqa: E731
+    back = lambda t: torch.where(live[:, :, None, None], t.permute(0, 2, 1, 3), 0.0).to(q.dtype).contiguous()  # noqa: E731
     qf, kvf = rows(q), rows(kv)
     kf = torch.cat([kvf[..., :dn], rows(k_rope.unsqueeze(2)).expand(B, H, S, dr)], -1)
     ok = live[:, None, :] & live[:, :, None]
     if causal:
         ok = ok & torch.ones(S, S, dtype=torch.bool, device=q.device).tril()
     p, lse = softmax_lse((torch.matmul(qf, kf.transpose(-1, -2)) * scale).masked_fill(~ok.unsqueeze(1), float("-inf")))
-    return qf, kf, kvf[..., dn:], p, lse, rows
+    return qf, kf, kvf[..., dn:], p, lse, rows, back
 
 
 def latent_attn_fwd(q: torch.Tensor, kv: torch.Tensor, k_rope: torch.Tensor, softmax_scale: Optional[float] = None,
@@ -75,8 +77,8 @@ def latent_attn_fwd(q: torch.Tensor, kv: torch.Tensor, k_rope: torch.Tensor, sof
     scale = _scale(q, softmax_scale)
     if use_native(q):
         return hip_ops().latent_attn_fwd(q, kv, k_rope, scale, causal, lens)
-    _, _, v, p, lse, _ = _ref_parts(q, kv, k_rope, scale, causal, lens)
-    return torch.matmul(p, v).permute(0, 2, 1, 3).to(q.dtype).contiguous(), lse
+    _, _, v, p, lse, _, back = _ref_parts(q, kv, k_rope, scale, causal, lens)
+    return back(torch.matmul(p, v)), lse
 
 
 def latent_attn_bwd(dout: torch.Tensor, q: torch.Tensor, kv: torch.Tensor, k_rope: torch.Tensor, out: torch.Tensor,
@@ -87,13 +89,12 @@ def latent_attn_bwd(dout: torch.Tensor, q: torch.Tensor, kv: torch.Tensor, k_rop
     if use_native(q):
         return hip_ops().latent_attn_bwd(dout, q, kv, k_rope, out, lse, scale, causal, lens)
     dn = _dims(q, kv, k_rope)[0]
-    qf, kf, v, p, _, rows = _ref_parts(q, kv, k_rope, scale, causal, lens)
+    qf, kf, v, p, _, rows, back = _ref_parts(q, kv, k_rope, scale, causal, lens)
     do, o = rows(dout), rows(out)
     ds = p * (torch.matmul(do, v.transpose(-1, -2)) - (do * o).sum(-1, keepdim=True)) * scale
     dk = torch.matmul(ds.transpose(-1, -2), qf)
     dkv = torch.cat([dk[..., :dn], torch.matmul(p.transpose(-1, -2), do)], -1)
-    back = lambda t: t.permute(0, 2, 1, 3).to(q.dtype).contiguous()  # noqa: E731
-    return back(torch.matmul(ds, kf)), back(dkv), dk[..., dn:].sum(1).to(q.dtype)
+    return back(torch.matmul(ds, kf)), back(dkv), back(dk[..., dn:].sum(1, keepdim=True)).squeeze(2)
 
 
 def once(grads: Tuple[torch.Tensor, ...], inputs: Tuple[torch.Tensor, ...]) -> Tuple[torch.Tensor, ...]:

@@ -54,13 +54,14 @@ def _ref_parts(q, k, v, pk, pv, scale, causal, lens, plens):
     vf, _ = _ref_keys(v, pv, lens, plens, rep)
     row = live_rows(lens, B, S, q.device)
     rows = lambda t: torch.where(row[:, :, None, None], t.to(kf.dtype), 0.0).permute(0, 2, 1, 3)  # noqa: E731
+    back = lambda t: torch.where(row[:, :, None, None], t.permute(0, 2, 1, 3), 0.0).to(q.dtype).contiguous()  # noqa: E731
     qf = rows(q)
     ok = live[:, None, :] & row[:, :, None]
     if causal:
         own = torch.ones(S, S, dtype=torch.bool, device=q.device).tril()
         ok = ok & torch.cat([own.new_ones(S, P), own], 1)
     p, lse = softmax_lse((torch.matmul(qf, kf.transpose(-1, -2)) * scale).masked_fill(~ok.unsqueeze(1), float("-inf")))
-    return qf, kf, vf, p, lse, rows
+    return qf, kf, vf, p, lse, rows, back
 
 
 def prefix_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor,
@@ -72,8 +73,8 @@ def prefix_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prefix_k:
     scale = _scale(q, softmax_scale)
     if use_native(q):
         return hip_ops().prefix_attn_fwd(q, k, v, prefix_k, prefix_v, scale, causal, lens, prefix_lens)
-    _, _, vf, p, lse, _ = _ref_parts(q, k, v, prefix_k, prefix_v, scale, causal, lens, prefix_lens)
-    return torch.matmul(p, vf).permute(0, 2, 1, 3).to(q.dtype).contiguous(), lse
+    _, _, vf, p, lse, _, back = _ref_parts(q, k, v, prefix_k, prefix_v, scale, causal, lens, prefix_lens)
+    return back(torch.matmul(p, vf)), lse
 
 
 def prefix_attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prefix_k: torch.Tensor,
@@ -86,17 +87,20 @@ def prefix_attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
         return hip_ops().prefix_attn_bwd(dout, q, k, v, prefix_k, prefix_v, out, lse, scale, causal, lens, prefix_lens)
     B, S, Hq, D = q.shape
     G, P, Hkv = prefix_k.shape[:3]
-    qf, kf, vf, p, _, rows = _ref_parts(q, k, v, prefix_k, prefix_v, scale, causal, lens, prefix_lens)
+    qf, kf, vf, p, _, rows, back = _ref_parts(q, k, v, prefix_k, prefix_v, scale, causal, lens, prefix_lens)
     do, o = rows(dout), rows(out)
     ds = p * (torch.matmul(do, vf.transpose(-1, -2)) - (do * o).sum(-1, keepdim=True)) * scale
 
+    some = live_rows(prefix_lens, G, P, q.device)[:, :, None, None]
+
     def split(t):  # [B, Hq, P + S, D] -> (own [B, S, Hkv, D], prefix [G, P, Hkv, D])
-        t = t.view(B, Hkv, Hq // Hkv, P + S, D).sum(2).permute(0, 2, 1, 3)
-        return t[:, P:].to(q.dtype).contiguous(), t[:, :P].reshape(G, B // G, P, Hkv, D).sum(1).to(q.dtype)
+        t = t.view(B, Hkv, Hq // Hkv, P + S, D).sum(2)
+        of_prefix = t[:, :, :P].permute(0, 2, 1, 3).reshape(G, B // G, P, Hkv, D).sum(1)
+        return back(t[:, :, P:]), torch.where(some, of_prefix, 0.0).to(q.dtype)
 
     dk, dpk = split(torch.matmul(ds.transpose(-1, -2), qf))
     dv, dpv = split(torch.matmul(p.transpose(-1, -2), do))
-    return torch.matmul(ds, kf).permute(0, 2, 1, 3).to(q.dtype).contiguous(), dk, dv, dpk, dpv
+    return back(torch.matmul(ds, kf)), dk, dv, dpk, dpv
 
 
 class PrefixAttentionFunction(torch.autograd.Function):

@@ -294,6 +294,39 @@ def _latent_args(dev, dt=torch.bfloat16, B=2, S=8, H=2, layout=HALF):
 
 
 @pytest.mark.parametrize("dev", [CPU, pytest.param(GPU, marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("S,causal", [(70, True), (150, False)])
+def test_rows_behind_a_length_are_zeros_beside_a_nan(dev, S, causal):
+    """NaN and infinity in live rows stay out of the rows that do not exist."""
+    g = torch.Generator().manual_seed(19)
+    lens, plens = [S - 9, 0, 5], [70]
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    alive, palive = live(lens, 3, S, dev), live(plens, 1, 90, dev)
+
+    def behind(*tensors):
+        for t, a in tensors:
+            assert not t[~a].any()
+
+    q, kv, kr = _latent_args(dev, B=3, S=S)
+    do = rnd(g, 3, S, 2, 64, dt=torch.bfloat16, dev=dev)
+    for t, bad in ((q, float("nan")), (kv, float("inf")), (kr, float("nan")), (do, float("nan"))):
+        t[0, 2, ..., 3] = bad
+        out, lse = ops.latent_attn_fwd(q, kv, kr, causal=causal, lens=i32(lens))
+        assert (lse.transpose(1, 2)[~alive] == float("-inf")).all()
+        dq, dkv, dkr = ops.latent_attn_bwd(do, q, kv, kr, out, lse, causal=causal, lens=i32(lens))
+        behind(*((x, alive) for x in (out, dq, dkv, dkr)))
+        t[0, 2] = 1
+    q, k, v, do = (rnd(g, 3, S, h, 64, dt=torch.bfloat16, dev=dev) for h in (4, 2, 2, 4))
+    pk, pv = (rnd(g, 1, 90, 2, 64, dt=torch.bfloat16, dev=dev) for _ in range(2))
+    for t, bad in ((q, float("nan")), (k, float("inf")), (v, float("nan")), (pk, float("nan")), (pv, float("inf")), (do, float("nan"))):
+        t[0, 2, 0, 3] = bad
+        out, lse = ops.prefix_attn_fwd(q, k, v, pk, pv, None, causal, i32(lens), i32(plens))
+        assert (lse.transpose(1, 2)[~alive] == float("-inf")).all()
+        dq, dk, dv, dpk, dpv = ops.prefix_attn_bwd(do, q, k, v, pk, pv, out, lse, None, causal, i32(lens), i32(plens))
+        behind((out, alive), (dq, alive), (dk, alive), (dv, alive), (dpk, palive), (dpv, palive))
+        t[0, 2] = 1
+
+
+@pytest.mark.parametrize("dev", [CPU, pytest.param(GPU, marks=pytest.mark.gpu)])
 def test_shapes_that_do_not_fit_are_refused(dev):
     q, kv, kr = _latent_args(dev)
     c, w = torch.zeros(2, 8, 16, dtype=q.dtype, device=dev), torch.zeros(2 * 128, 16, dtype=q.dtype, device=dev)
