@@ -48,8 +48,31 @@ def _dims(q: torch.Tensor, kv: torch.Tensor, k_rope: torch.Tensor) -> Tuple[int,
     return dn, dr, kv.shape[-1] - dn
 
 
-def _scale(q: torch.Tensor, softmax_scale: Optional[float]) -> float:
-    return softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(q.shape[-1])
+def scale_of(q: torch.Tensor, softmax_scale: Optional[float]) -> float:
+    scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(q.shape[-1])
+    if not 1e-20 <= scale <= 1e20:
+        raise ValueError(f"softmax_scale must lie between 1e-20 and 1e20, got {scale}")
+    return scale
+
+
+def check_reference(op: str, fits: bool, tensors: Tuple[torch.Tensor, ...], *lengths: Tuple[Lens, int]) -> None:
+    """What the kernels refuse is refused by the reference, too: shapes that would broadcast, mixed types, lengths of another
+    type or number."""
+    q = tensors[0]
+    if not fits:
+        raise ValueError(f"{op}: shapes {', '.join(str(tuple(t.shape)) for t in tensors)} do not fit together")
+    if any(t.dtype != q.dtype or t.device != q.device for t in tensors):
+        raise ValueError(f"{op}: all tensors must share q's device and type")
+    for lens, n in lengths:
+        if lens is not None and not (lens.dtype == torch.int32 and lens.shape == (n,) and lens.device == q.device):
+            raise ValueError(f"{op}: lengths must be an int32 tensor [{n}] on q's device, got {lens.dtype} {tuple(lens.shape)}")
+
+
+def _check_latent(op, q, kv, k_rope, lens, *outs):
+    fits = q.dim() == kv.dim() == 4 and k_rope.dim() == 3 and kv.shape[:3] == q.shape[:3] and k_rope.shape[:2] == q.shape[:2] \
+        and 0 <= q.shape[3] - k_rope.shape[2] < kv.shape[3]
+    fits = fits and all(t.shape == (*q.shape[:3], _dims(q, kv, k_rope)[2]) for t in outs)
+    check_reference(op, fits, (q, kv, k_rope, *outs), (lens, q.shape[0]))
 
 
 def _ref_parts(q, kv, k_rope, scale, causal, lens):
@@ -74,9 +97,10 @@ def latent_attn_fwd(q: torch.Tensor, kv: torch.Tensor, k_rope: torch.Tensor, sof
                     causal: bool = True, lens: Lens = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """q [B, S, H, nope + rope], kv [B, S, H, nope + value], k_rope [B, S, rope] -> (out [B, S, H, value] contiguous,
     log-sum-exp fp32 [B, H, S])."""
-    scale = _scale(q, softmax_scale)
+    scale = scale_of(q, softmax_scale)
     if use_native(q):
         return hip_ops().latent_attn_fwd(q, kv, k_rope, scale, causal, lens)
+    _check_latent("latent_attn_fwd", q, kv, k_rope, lens)
     _, _, v, p, lse, _, back = _ref_parts(q, kv, k_rope, scale, causal, lens)
     return back(torch.matmul(p, v)), lse
 
@@ -85,9 +109,10 @@ def latent_attn_bwd(dout: torch.Tensor, q: torch.Tensor, kv: torch.Tensor, k_rop
                     lse: torch.Tensor, softmax_scale: Optional[float] = None, causal: bool = True,
                     lens: Lens = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(dq, dkv, dk_rope), contiguous; dk_rope is summed over the heads in fp32. ``out`` and ``lse`` are the forward's."""
-    scale = _scale(q, softmax_scale)
+    scale = scale_of(q, softmax_scale)
     if use_native(q):
         return hip_ops().latent_attn_bwd(dout, q, kv, k_rope, out, lse, scale, causal, lens)
+    _check_latent("latent_attn_bwd", q, kv, k_rope, lens, dout, out)
     dn = _dims(q, kv, k_rope)[0]
     qf, kf, v, p, _, rows, back = _ref_parts(q, kv, k_rope, scale, causal, lens)
     do, o = rows(dout), rows(out)
@@ -141,7 +166,7 @@ def latent_attention(q: torch.Tensor, c: torch.Tensor, k_rope: torch.Tensor, w_k
         raise ValueError(f"latent_attention: q {tuple(q.shape)}, c {tuple(c.shape)}, k_rope {tuple(k_rope.shape)} and "
                          f"w_kv {tuple(w_kv.shape)} do not fit together")
     if use_native(q):  # the same composition as one operator each way (csrc/autograd.cpp)
-        return hip_ops().latent_attention(q, c, k_rope, w_kv, _scale(q, softmax_scale), causal, lens)
+        return hip_ops().latent_attention(q, c, k_rope, w_kv, scale_of(q, softmax_scale), causal, lens)
     return LatentAttentionFunction.apply(q, c, k_rope, w_kv, softmax_scale, causal, lens)
 
 
@@ -149,9 +174,12 @@ def latent_attention_decode(q: torch.Tensor, cache: torch.Tensor, lens: torch.Te
                             softmax_scale: Optional[float] = None) -> torch.Tensor:
     """One token per sequence: q [B, H, nope + rope] over cache [B, L, r + rope] (per token the latent vector, then the
     rope key; the token's own row already stored), lens int32 [B] -> out [B, H, value]. A sequence of length 0 gives zeros."""
-    scale = _scale(q, softmax_scale)
+    scale = scale_of(q, softmax_scale)
     if use_native(q):
         return hip_ops().latent_attn_decode(q, cache, lens, w_kv, scale)
+    fits = q.dim() == cache.dim() == 3 and w_kv.dim() == 2 and cache.shape[0] == q.shape[0] and q.shape[1] > 0 \
+        and w_kv.shape[0] % q.shape[1] == 0 and 0 <= cache.shape[2] - w_kv.shape[1] <= q.shape[2]
+    check_reference("latent_attention_decode", fits, (q, cache, w_kv), (lens, q.shape[0]))
     B, H, d = q.shape
     r, L = w_kv.shape[1], cache.shape[1]
     dn = d - (cache.shape[-1] - r)

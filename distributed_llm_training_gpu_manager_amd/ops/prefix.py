@@ -14,17 +14,12 @@ behind may hold anything; outputs and gradients there are zeros, the log-sum-exp
 """
 from __future__ import annotations
 
-import math
 from typing import Optional, Tuple
 
 import torch
 
 from .._native import hip_ops, use_native
-from .latent import Lens, live_rows, once, softmax_lse
-
-
-def _scale(q: torch.Tensor, softmax_scale: Optional[float]) -> float:
-    return softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(q.shape[-1])
+from .latent import Lens, check_reference, live_rows, once, scale_of, softmax_lse
 
 
 def _check(q, k, prefix_k):
@@ -33,6 +28,13 @@ def _check(q, k, prefix_k):
         raise ValueError(f"prefix attention: a batch of {B} does not hold equally many sequences of {G} prefixes")
     if not Hkv or Hq % Hkv or prefix_k.shape[2] != Hkv:
         raise ValueError(f"prefix attention: {Hq} q heads, {Hkv} kv heads, {prefix_k.shape[2]} prefix kv heads")
+
+
+def _check_reference(op, q, k, v, pk, pv, lens, plens, *outs):
+    fits = k.dim() == v.dim() == pk.dim() == pv.dim() == 4 and k.shape[0] == q.shape[0] and k.shape[3] == q.shape[-1] \
+        and v.shape == k.shape and pk.shape[2:] == k.shape[2:] and pv.shape == pk.shape
+    fits = fits and (q.dim() == 3 or q.dim() == 4 and k.shape[1] == q.shape[1]) and all(t.shape == q.shape for t in outs)
+    check_reference(op, fits, (q, k, v, pk, pv, *outs), (lens, q.shape[0]), (plens, pk.shape[0]))
 
 
 def _ref_keys(x, px, lens, plens, rep):
@@ -70,9 +72,10 @@ def prefix_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prefix_k:
     """q [B, S, Hq, D], k / v [B, S, Hkv, D], prefix_k / prefix_v [G, P, Hkv, D] -> (out [B, S, Hq, D] contiguous,
     log-sum-exp fp32 [B, Hq, S]). ``causal`` concerns a sequence's own keys; its prefix is always seen whole."""
     _check(q, k, prefix_k)
-    scale = _scale(q, softmax_scale)
+    scale = scale_of(q, softmax_scale)
     if use_native(q):
         return hip_ops().prefix_attn_fwd(q, k, v, prefix_k, prefix_v, scale, causal, lens, prefix_lens)
+    _check_reference("prefix_attn_fwd", q, k, v, prefix_k, prefix_v, lens, prefix_lens)
     _, _, vf, p, lse, _, back = _ref_parts(q, k, v, prefix_k, prefix_v, scale, causal, lens, prefix_lens)
     return back(torch.matmul(p, vf)), lse
 
@@ -82,9 +85,10 @@ def prefix_attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
                     causal: bool = True, lens: Lens = None, prefix_lens: Lens = None):
     """(dq, dk, dv, dprefix_k, dprefix_v), contiguous. ``out`` and ``lse`` are the forward's."""
     _check(q, k, prefix_k)
-    scale = _scale(q, softmax_scale)
+    scale = scale_of(q, softmax_scale)
     if use_native(q):
         return hip_ops().prefix_attn_bwd(dout, q, k, v, prefix_k, prefix_v, out, lse, scale, causal, lens, prefix_lens)
+    _check_reference("prefix_attn_bwd", q, k, v, prefix_k, prefix_v, lens, prefix_lens, dout, out)
     B, S, Hq, D = q.shape
     G, P, Hkv = prefix_k.shape[:3]
     qf, kf, vf, p, _, rows, back = _ref_parts(q, k, v, prefix_k, prefix_v, scale, causal, lens, prefix_lens)
@@ -124,7 +128,7 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prefix_k
     """out [B, S, Hq, D] as :func:`prefix_attn_fwd`, differentiable in q, k, v, prefix_k and prefix_v."""
     _check(q, k, prefix_k)
     if use_native(q):  # one operator each way (csrc/autograd.cpp)
-        return hip_ops().prefix_attention(q, k, v, prefix_k, prefix_v, _scale(q, softmax_scale), causal, lens, prefix_lens)
+        return hip_ops().prefix_attention(q, k, v, prefix_k, prefix_v, scale_of(q, softmax_scale), causal, lens, prefix_lens)
     return PrefixAttentionFunction.apply(q, k, v, prefix_k, prefix_v, softmax_scale, causal, lens, prefix_lens)
 
 
@@ -134,9 +138,10 @@ def prefix_attention_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, l
     """One token per sequence: q [B, Hq, D] over the group's prefix and the sequence's own cache k / v [B, L, Hkv, D] of
     lens int32 [B] tokens (the token's own row already stored) -> out [B, Hq, D]. No keys at all give zeros."""
     _check(q, k, prefix_k)
-    scale = _scale(q, softmax_scale)
+    scale = scale_of(q, softmax_scale)
     if use_native(q):
         return hip_ops().prefix_attn_decode(q, k, v, lens, prefix_k, prefix_v, scale, prefix_lens)
+    _check_reference("prefix_attention_decode", q, k, v, prefix_k, prefix_v, lens, prefix_lens)
     rep = q.shape[1] // k.shape[2]
     kf, live = _ref_keys(k, prefix_k, lens, prefix_lens, rep)
     vf, _ = _ref_keys(v, prefix_v, lens, prefix_lens, rep)

@@ -342,6 +342,53 @@ def test_shapes_that_do_not_fit_are_refused(dev):
             ops.prefix_attention_decode(args[0][:, 0], *args[1:3], torch.zeros(6, dtype=torch.int32, device=dev), *args[3:])
 
 
+@pytest.mark.parametrize("dev", [CPU, pytest.param(GPU, marks=pytest.mark.gpu)])
+def test_reference_and_kernels_refuse_the_same(dev):
+    """Shapes that would broadcast, mixed types, lengths of another type or number, scales without a softmax."""
+    q, kv, kr = _latent_args(dev)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    out, lse = ops.latent_attn_fwd(q, kv, kr, lens=i32(8, 3))
+    cache, w = torch.zeros(2, 9, 256 + 32, dtype=q.dtype, device=dev), torch.zeros(2 * 128, 256, dtype=q.dtype, device=dev)
+    pq, k, pk = (torch.zeros(*s, dtype=q.dtype, device=dev) for s in ((4, 8, 4, 64), (4, 8, 2, 64), (2, 5, 2, 64)))
+    po, plse = ops.prefix_attn_fwd(pq, k, k, pk, pk, lens=i32(1, 2, 3, 4), prefix_lens=i32(5, 0))
+    ops.latent_attn_bwd(out, q, kv, kr, out, lse, lens=i32(8, 3)), ops.prefix_attn_bwd(po, pq, k, k, pk, pk, po, plse)
+    ops.latent_attention_decode(q[:, 0], cache, i32(1, 2), w), ops.prefix_attention_decode(pq[:, 0], k, k, i32(1, 2, 3, 4), pk, pk)
+    bad = [
+        lambda: ops.latent_attn_fwd(q, kv[:1], kr),
+        lambda: ops.latent_attn_fwd(q, kv, kr[:, :1]),
+        lambda: ops.latent_attn_fwd(q, kv[:, :, :1], kr),
+        lambda: ops.latent_attn_fwd(q.half(), kv, kr),
+        lambda: ops.latent_attn_fwd(q, kv, kr, lens=i32(8, 8).long()),
+        lambda: ops.latent_attn_fwd(q, kv, kr, lens=i32(8)),
+        lambda: ops.latent_attn_fwd(q, kv, kr, lens=i32(8, 8).view(2, 1)),
+        lambda: ops.latent_attn_bwd(out[:1], q, kv, kr, out, lse),
+        lambda: ops.latent_attn_bwd(out, q, kv, kr, out[:, :1], lse),
+        lambda: ops.latent_attention_decode(q[:, 0], cache[:1], i32(1, 2), w),
+        lambda: ops.latent_attention_decode(q[:, 0], cache, i32(1, 2).long(), w),
+        lambda: ops.latent_attention_decode(q[:, 0], cache, i32(1), w),
+        lambda: ops.latent_attention_decode(q[:, 0], cache, i32(1, 2), w[:-1]),
+        lambda: ops.prefix_attn_fwd(pq, k, k[:, :4], pk, pk),
+        lambda: ops.prefix_attn_fwd(pq, k[:1], k[:1], pk, pk),
+        lambda: ops.prefix_attn_fwd(pq, k[:, :1], k[:, :1], pk, pk),
+        lambda: ops.prefix_attn_fwd(pq, k, k, pk, pk[:1]),
+        lambda: ops.prefix_attn_fwd(pq, k, k.half(), pk, pk),
+        lambda: ops.prefix_attn_fwd(pq, k, k, pk, pk, lens=i32(1, 2, 3)),
+        lambda: ops.prefix_attn_fwd(pq, k, k, pk, pk, prefix_lens=i32(1)),
+        lambda: ops.prefix_attn_bwd(po[:1], pq, k, k, pk, pk, po, plse),
+        lambda: ops.prefix_attention_decode(pq[:, 0], k, k, i32(1, 2, 3, 4).long(), pk, pk),
+        lambda: ops.prefix_attention_decode(pq[:, 0], k, k[:1], i32(1, 2, 3, 4), pk, pk),
+    ]
+    for scale in (0.0, -1.0, 1e-30, 1e30, float("nan"), float("inf")):
+        bad += [lambda x=scale: ops.latent_attn_fwd(q, kv, kr, x), lambda x=scale: ops.latent_attn_bwd(out, q, kv, kr, out, lse, x),
+                lambda x=scale: ops.latent_attention_decode(q[:, 0], cache, i32(1, 2), w, x),
+                lambda x=scale: ops.prefix_attn_fwd(pq, k, k, pk, pk, x), lambda x=scale: ops.prefix_attn_bwd(po, pq, k, k, pk, pk, po, plse, x),
+                lambda x=scale: ops.prefix_attention_decode(pq[:, 0], k, k, i32(1, 2, 3, 4), pk, pk, None, x)]
+    for i, call in enumerate(bad):
+        with pytest.raises((RuntimeError, ValueError)):
+            call()
+            pytest.fail(f"call {i} was not refused")
+
+
 # ---- the kernels (GPU) -------------------------------------------------------------------------
 
 BF, FP = torch.bfloat16, torch.float16
