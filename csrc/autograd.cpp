@@ -8,6 +8,8 @@
 #include <torch/library.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <hip/hip_runtime.h>
 
 using torch::autograd::AutogradContext;
 using torch::autograd::Variable;
@@ -103,6 +105,23 @@ auto op(const char* name) {
   return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
 }
 
+// A backward that is captured while an eager graph of the same leaves is alive: the leaves' accumulation was then recorded
+// on the default stream, which torch's engine would make wait for this node's gradients. The default stream cannot join a
+// capture, and the engine ends the process over it; raised here instead, before a kernel is launched.
+void check_capture(const char* op) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  const bool asked = hipStreamIsCapturing(c10::hip::getCurrentHIPStream(), &status) == hipSuccess;
+  const auto node = torch::autograd::get_current_node();
+  if (!asked || status != hipStreamCaptureStatusActive || !node) return;
+  for (const auto& edge : node->next_edges()) {
+    if (!edge.is_valid()) continue;
+    const auto next = edge.function->stream();
+    TORCH_CHECK(!next || c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, *next).stream() != nullptr, op,
+                ": this backward is captured into a graph, but a graph recorded on the default stream holds the same inputs; "
+                "release it (its outputs) first, or record it on the capture's stream");
+  }
+}
+
 // Gradients recorded for a second differentiation (create_graph) with regard to the inputs raise an error there: no kernel
 // has a second derivative. `all`: as many entries as the forward has arguments, the gradients first.
 variable_list once(variable_list grads, const Variable& dout, const variable_list& saved, size_t all) {
@@ -131,6 +150,7 @@ struct LatentAttention : public torch::autograd::Function<LatentAttention> {
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list dout) {
+    check_capture("latent_attention");
     const auto s = ctx->get_saved_variables();
     at::AutoDispatchBelowADInplaceOrView below;
     static auto bwd = op<decltype(latent_attention_bwd)>("dlgm::latent_attention_bwd");
@@ -162,6 +182,7 @@ struct PrefixAttention : public torch::autograd::Function<PrefixAttention> {
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list dout) {
+    check_capture("prefix_attention");
     const auto s = ctx->get_saved_variables();
     at::AutoDispatchBelowADInplaceOrView below;
     static auto bwd = op<PrefixBwd>("dlgm::prefix_attn_bwd");

@@ -668,6 +668,41 @@ def test_differentiable_calls_are_captured():
 
 
 @pytest.mark.gpu
+def test_capture_of_a_backward_beside_an_eager_graph_is_refused():
+    """The engine would make the default stream, on which the eager graph recorded the leaves' accumulation, wait for a
+    captured kernel. The call raises, the capture goes on, and the backward is captured once the eager graph is gone."""
+    q, c, kr, w, do = (t.requires_grad_(i < 4) for i, t in enumerate(_train_inputs(20)))
+    g = torch.Generator().manual_seed(21)
+    x = [rnd(g, *s, dt=BF, dev=GPU).requires_grad_(True) for s in ((2, 40, 4, 64), (2, 40, 2, 64), (2, 40, 2, 64), (1, 90, 2, 64), (1, 90, 2, 64))]
+    xdo = rnd(g, 2, 40, 4, 64, dt=BF, dev=GPU)
+    for fn, leaves, grad, name in ((ops.latent_attention, (q, c, kr, w), do, "latent_attention"), (ops.prefix_attention, x, xdo, "prefix_attention")):
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            torch.autograd.grad(fn(*leaves), leaves, grad)
+        torch.cuda.current_stream().wait_stream(s)
+        eager = fn(*leaves)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=s):
+            out = fn(*leaves)
+            with pytest.raises(RuntimeError, match=name + ": this backward is captured"):
+                torch.autograd.grad(out, leaves, grad)
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
+        want = torch.autograd.grad(eager, leaves, grad)
+        del eager, out, gr
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=s):
+            got = torch.autograd.grad(fn(*leaves), leaves, grad)
+        for _ in range(2):
+            gr.replay()
+            torch.cuda.synchronize()
+            u = torch.finfo(BF).eps / 2  # a GEMM may be another one on the stream's own workspace
+            assert all(float((a.double() - b.double()).norm()) <= 2 * u * float(b.double().norm()) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
 def test_odd_arguments():
     """Lengths outside the tensors' count as their ends; views that a GEMM cannot read in place; no gradient to record."""
     q, c, kr, w, do = _train_inputs(14)
