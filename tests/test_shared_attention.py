@@ -511,6 +511,74 @@ def test_latent_attention_is_its_parts():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("causal,scale,lens,plens", [
+    (True, None, None, None), (False, 0.3, [40, 7, 0, 33], [90, 31]), (True, 0.05, [40, 40, 1, 12], None), (False, None, None, [0, 90])])
+def test_prefix_attention_is_its_parts(causal, scale, lens, plens):
+    """The differentiable entry point is the kernel pair, bit for bit, each argument in its place."""
+    g = torch.Generator().manual_seed(22)
+    x = [rnd(g, *s, dt=BF, dev=GPU) for s in ((4, 40, 4, 64), (4, 40, 2, 64), (4, 40, 2, 64), (2, 90, 2, 64), (2, 90, 2, 64))]
+    do = rnd(g, 4, 40, 4, 64, dt=BF, dev=GPU)
+    lt, pt = (None if n is None else torch.tensor(n, dtype=torch.int32, device=GPU) for n in (lens, plens))
+    leaves = [t.clone().requires_grad_(True) for t in x]
+    out = ops.prefix_attention(*leaves, scale, causal, lt, pt)
+    o, lse = ops.prefix_attn_fwd(*x, scale, causal, lt, pt)
+    assert torch.equal(out, o)
+    want = ops.prefix_attn_bwd(do, *x, o, lse, scale, causal, lt, pt)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, leaves, do), want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,layout,r,causal,scale,lens", [
+    (FP, HALF, 512, False, 0.2, [100, 41]), (BF, WIDE, 512, True, 0.02, None), (FP, WIDE, 256, False, None, [99, 0]),
+    (BF, HALF, 256, True, 0.3, [1, 100])])
+def test_latent_attention_against_the_reference(dt, layout, r, causal, scale, lens):
+    """Both types and layouts, with and without a mask, a scale and lengths. Roundings on the way as above (6 u); scores s
+    from the rounded up-projection are off by u |s| each, a weight and its sum by that factor: 2 u max |s| more."""
+    dn, dr, dv = layout
+    B, S, H = 2, 100, 3
+    g = torch.Generator().manual_seed(23)
+    x = [rnd(g, *s, dt=dt, dev=GPU) for s in ((B, S, H, dn + dr), (B, S, r), (B, S, dr))]
+    x.append(rnd(g, H * (dn + dv), r, dt=dt, dev=GPU, std=r ** -0.5))
+    do = rnd(g, B, S, H, dv, dt=dt, dev=GPU)
+    lt = None if lens is None else torch.tensor(lens, dtype=torch.int32)
+    leaves = [t.clone().requires_grad_(True) for t in x]
+    out = ops.latent_attention(*leaves, scale, causal, None if lt is None else lt.to(GPU))
+    got = (out, *torch.autograd.grad(out, leaves, do))
+    ref = [t.cpu().double().requires_grad_(True) for t in x]
+    ro = ops.latent_attention(*ref, scale, causal, lt)
+    want = (ro, *torch.autograd.grad(ro, ref, do.cpu().double()))
+    kv = (ref[1].detach() @ ref[3].detach().t()).view(B, S, H, -1)
+    s = torch.einsum("bihd,bjhd->bhij", ref[0].detach(), torch.cat([kv[..., :dn], ref[2].detach().unsqueeze(2).expand(B, S, H, dr)], -1))
+    u = torch.finfo(dt).eps / 2
+    allow = (6 + 2 * float(s.abs().max()) * (scale or (dn + dr) ** -0.5)) * u
+    for a, b in zip(got, want):
+        assert float((a.detach().cpu().double() - b.detach()).norm()) <= allow * float(b.detach().norm())
+
+
+@pytest.mark.gpu
+def test_large_weight_gradient():
+    """8192 tokens and weights of 32 x 256 rows: dw_kv is a product with c transposed first. dc and dw_kv against dkv w_kv and
+    dkv^T c in 64 bits: an fp32 chain of 8192 terms and one rounding."""
+    B, S, H, (dn, dr, dv), r = 16, 512, 32, WIDE, 512
+    g = torch.Generator(device=GPU).manual_seed(24)
+    q, c, kr, w, do = (torch.randn(*s, generator=g, device=GPU) for s in ((B, S, H, dn + dr), (B, S, r), (B, S, dr), (H * (dn + dv), r), (B, S, H, dv)))
+    q, c, kr, w, do = (t.to(BF) for t in (q, c, kr, w * r ** -0.5, do))
+    leaves = [t.requires_grad_(True) for t in (q, c, kr, w)]
+    out = ops.latent_attention(*leaves)
+    dq, dc, dkr, dw = torch.autograd.grad(out, leaves, do)
+    q, c, kr, w = (t.detach() for t in leaves)
+    kv = torch.empty(B, S, H, dn + dv, dtype=BF, device=GPU)
+    torch.ops.dlgm.gemm_lt(kv.view(B * S, -1), c.view(B * S, r), w.t(), 0.0, -1)
+    o, lse = ops.latent_attn_fwd(q, kv, kr)
+    want = ops.latent_attn_bwd(do, q, kv, kr, o, lse)
+    assert torch.equal(out.detach(), o) and torch.equal(dq, want[0]) and torch.equal(dkr, want[2])
+    d2, c2, u = want[1].view(B * S, -1).double(), c.view(B * S, r).double(), torch.finfo(BF).eps / 2
+    for got, a, b in ((dw, d2.t().contiguous(), c2), (dc.view(B * S, r), d2, w.double())):
+        exact = a @ b
+        assert ((got.double() - exact).abs() <= u * exact.abs() + (1 + u) * 8192 * F32 * (a.abs() @ b.abs())).all()
+
+
+@pytest.mark.gpu
 def test_training_and_sampling_of_a_group():
     """As used together: answers sampled token by token over a shared prefix get the outputs that the training form gives
     the whole answers, and the same for a latent cache."""
