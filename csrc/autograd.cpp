@@ -109,10 +109,12 @@ auto op(const char* name) {
 // on the default stream, which torch's engine would make wait for this node's gradients. The default stream cannot join a
 // capture, and the engine ends the process over it; raised here instead, before a kernel is launched.
 void check_capture(const char* op) {
-  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-  const bool asked = hipStreamIsCapturing(c10::hip::getCurrentHIPStream(), &status) == hipSuccess;
+  const hipStream_t stream = c10::hip::getCurrentHIPStream();
   const auto node = torch::autograd::get_current_node();
-  if (!asked || status != hipStreamCaptureStatusActive || !node) return;
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (stream == nullptr || !node || hipStreamIsCapturing(stream, &status) != hipSuccess ||
+      status != hipStreamCaptureStatusActive)
+    return;
   for (const auto& edge : node->next_edges()) {
     if (!edge.is_valid()) continue;
     const auto next = edge.function->stream();
