@@ -63,7 +63,8 @@ at::Tensor rows16(const at::Tensor& t) {
   return reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 ? x : x.clone();
 }
 
-// kv = c w_kv^T by one dense GEMM, then the attention
+// kv = c w_kv^T by one dense GEMM, then the attention. kv is stored in the 16-bit type, rounded once from the product's fp32:
+// its rows are operands of the matrix units, which take no more, and twice the bytes would be read by every tile of queries
 std::tuple<at::Tensor, at::Tensor, at::Tensor> latent_attention_fwd(const at::Tensor& q, const at::Tensor& c,
                                                                     const at::Tensor& k_rope, const at::Tensor& w_kv,
                                                                     double softmax_scale, bool causal,
@@ -77,7 +78,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> latent_attention_fwd(const at::Te
   return {out, lse, kv};
 }
 
-// (dq, dc, dk_rope, dw_kv)
+// (dq, dc, dk_rope, dw_kv). dkv, the operand of both GEMMs, is rounded to the 16-bit type for the same reason
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> latent_attention_bwd(
     const at::Tensor& dout, const at::Tensor& q, const at::Tensor& c, const at::Tensor& k_rope, const at::Tensor& w_kv,
     const at::Tensor& kv, const at::Tensor& out, const at::Tensor& lse, double softmax_scale, bool causal,

@@ -228,7 +228,8 @@ __global__ __launch_bounds__(kThreads * SPLIT, 2) void shared_fwd_kernel(SharedA
 }
 
 // ---- dQ: one workgroup per (b, q head, 128 queries), the forward's walk and split. It holds dO in registers, so it also
-// forms delta and writes the [-delta, -lse/scale] rows the dK/dV pass starts its accumulators from (padded rows: 0, 0).
+// forms delta and writes the [-delta, -lse/scale] rows the dK/dV pass starts its accumulators from (padded rows: 0, 0). delta
+// is that of the output as stored, in 16 bits: the unrounded one would have to be kept in fp32 for every row.
 template <typename E, int DA, int DB, int DV, bool PRE, int SPLIT>
 __global__ __launch_bounds__(kThreads * SPLIT, 2) void shared_bwd_dq_kernel(SharedArgs<E> p) {
   constexpr int KA = DA / 16, KB = DB / 16, KK = KA + KB, KV = DV / 16, DT = (DA + DB) / 32;

@@ -12,7 +12,9 @@ heads come from ONE latent vector ``c`` [r] a token, plus one rope key ``k_rope`
 On the GPU: bf16 or fp16; head dims (nope, rope, value) (128, 64, 128) or (64, 32, 64); r any multiple of 8 in training, 256
 or 512 in the single-token form; strided views with 16-byte rows. ``lens`` (int32 [B], values beyond the tensor's length
 count as its length): only the first ``lens[b]`` tokens of sequence b exist. What lies behind them may hold anything; their
-outputs and gradients are zeros, their log-sum-exp is -inf. CPU tensors take the fp32 reference below.
+outputs and gradients are zeros, their log-sum-exp is -inf (:func:`latent_attention` alone reads every row of ``c`` in its
+GEMMs, so there they must be finite). A NaN in a live row may reach every other live row of its sequence. CPU tensors take the
+fp32 reference below, which refuses what the kernels refuse but for types, head dims and strides.
 """
 from __future__ import annotations
 

@@ -136,7 +136,8 @@ def prefix_attention_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, l
                             prefix_k: torch.Tensor, prefix_v: torch.Tensor, prefix_lens: Lens = None,
                             softmax_scale: Optional[float] = None) -> torch.Tensor:
     """One token per sequence: q [B, Hq, D] over the group's prefix and the sequence's own cache k / v [B, L, Hkv, D] of
-    lens int32 [B] tokens (the token's own row already stored) -> out [B, Hq, D]. No keys at all give zeros."""
+    lens int32 [B] tokens (the token's own row already stored) -> out [B, Hq, D]. No keys at all give zeros. The kernel's work is
+    cut by L and P, not by the lengths: pass views of a cache that is allocated well beyond its longest sequence."""
     _check(q, k, prefix_k)
     scale = scale_of(q, softmax_scale)
     if use_native(q):
