@@ -23,6 +23,11 @@ inline void check_rows(const at::Tensor& t, const at::Tensor& like, const char* 
   TORCH_CHECK(t.size(rd) <= 1 || t.stride(rd) < (int64_t)1 << 23, op, ": ", name, " row stride is too large");
 }
 
+// The stride of dimension i as the kernels use it. Of a dimension of one it may be anything (1 for a permuted [B, H, D, 1]):
+// rows a tile has beyond it are then placed a row's width apart, behind the end of the one that exists, where a descriptor
+// gives zeros and every address stays aligned.
+inline int64_t stride_of(const at::Tensor& t, int i) { return t.size(i) > 1 ? t.stride(i) : t.size(t.dim() - 1); }
+
 inline const int* check_lens(const c10::optional<at::Tensor>& lens, const at::Tensor& like, int64_t n, const char* op,
                              const char* name) {
   if (!lens.has_value() || !lens->defined()) return nullptr;

@@ -784,9 +784,9 @@ SharedArgs<E> latent_args(const at::Tensor& q, const at::Tensor& kv, const at::T
                           double scale, bool causal) {
   SharedArgs<E> p{};
   p.q = ptr<E>(q), p.k = ptr<E>(kv), p.v = ptr<E>(kv) + dn, p.kr = ptr<E>(kr);
-  p.q_sb = q.stride(0), p.q_ss = q.stride(1), p.q_sh = q.stride(2);
-  p.k_sb = p.v_sb = kv.stride(0), p.k_ss = p.v_ss = kv.stride(1), p.k_sh = p.v_sh = kv.stride(2);
-  p.kr_sb = kr.stride(0), p.kr_ss = kr.stride(1);
+  p.q_sb = stride_of(q, 0), p.q_ss = stride_of(q, 1), p.q_sh = stride_of(q, 2);
+  p.k_sb = p.v_sb = stride_of(kv, 0), p.k_ss = p.v_ss = stride_of(kv, 1), p.k_sh = p.v_sh = stride_of(kv, 2);
+  p.kr_sb = stride_of(kr, 0), p.kr_ss = stride_of(kr, 1);
   p.lens = lens;
   p.B = q.size(0), p.S = q.size(1), p.Hq = p.Hkv = q.size(2), p.n = 1;
   p.scale = scale, p.scale_log2 = scale * kLog2e, p.neg_inv_scale = -1.0 / scale;
@@ -817,11 +817,11 @@ SharedArgs<E> prefix_args(const at::Tensor& q, const at::Tensor& k, const at::Te
                           const at::Tensor& pv, const int* lens, const int* plens, double scale, bool causal) {
   SharedArgs<E> p{};
   p.q = ptr<E>(q), p.k = ptr<E>(k), p.v = ptr<E>(v), p.pk = ptr<E>(pk), p.pv = ptr<E>(pv);
-  p.q_sb = q.stride(0), p.q_ss = q.stride(1), p.q_sh = q.stride(2);
-  p.k_sb = k.stride(0), p.k_ss = k.stride(1), p.k_sh = k.stride(2);
-  p.v_sb = v.stride(0), p.v_ss = v.stride(1), p.v_sh = v.stride(2);
-  p.pk_sb = pk.stride(0), p.pk_ss = pk.stride(1), p.pk_sh = pk.stride(2);
-  p.pv_sb = pv.stride(0), p.pv_ss = pv.stride(1), p.pv_sh = pv.stride(2);
+  p.q_sb = stride_of(q, 0), p.q_ss = stride_of(q, 1), p.q_sh = stride_of(q, 2);
+  p.k_sb = stride_of(k, 0), p.k_ss = stride_of(k, 1), p.k_sh = stride_of(k, 2);
+  p.v_sb = stride_of(v, 0), p.v_ss = stride_of(v, 1), p.v_sh = stride_of(v, 2);
+  p.pk_sb = stride_of(pk, 0), p.pk_ss = stride_of(pk, 1), p.pk_sh = stride_of(pk, 2);
+  p.pv_sb = stride_of(pv, 0), p.pv_ss = stride_of(pv, 1), p.pv_sh = stride_of(pv, 2);
   p.lens = lens, p.plens = plens;
   p.B = q.size(0), p.S = q.size(1), p.Hq = q.size(2), p.Hkv = k.size(2), p.P = pk.size(1), p.n = p.B / pk.size(0);
   p.scale = scale, p.scale_log2 = scale * kLog2e, p.neg_inv_scale = -1.0 / scale;
@@ -892,7 +892,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> dlgm_latent_attn_bwd(const at::Te
   DLGM_DISPATCH_16(q.scalar_type(), E, {
     auto p = latent_args<E>(q, kv, k_rope, dn, lp, softmax_scale, causal);
     p.o = ptr<E>(out), p.dout = ptr<E>(dout), p.lse = lse.data_ptr<float>(), p.rows = rows.data_ptr<float>();
-    p.do_sb = dout.stride(0), p.do_ss = dout.stride(1), p.do_sh = dout.stride(2);
+    p.do_sb = stride_of(dout, 0), p.do_ss = stride_of(dout, 1), p.do_sh = stride_of(dout, 2);
     p.dq = ptr<E>(dq), p.dk = ptr<E>(dkv), p.dv = ptr<E>(dkv) + dn;
     p.dk_ss = p.dv_ss = H * (dn + dv), p.dk_sh = p.dv_sh = dn + dv;
     p.dkr_part = dkr_part.data_ptr<float>();
@@ -999,7 +999,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> dlgm_pref
   DLGM_DISPATCH_16(q.scalar_type(), E, {
     auto p = prefix_args<E>(q, k, v, prefix_k, prefix_v, lp, pp, softmax_scale, causal);
     p.o = ptr<E>(out), p.dout = ptr<E>(dout), p.lse = lse.data_ptr<float>(), p.rows = rows.data_ptr<float>();
-    p.do_sb = dout.stride(0), p.do_ss = dout.stride(1), p.do_sh = dout.stride(2);
+    p.do_sb = stride_of(dout, 0), p.do_ss = stride_of(dout, 1), p.do_sh = stride_of(dout, 2);
     p.dq = ptr<E>(dq), p.dk = ptr<E>(dk), p.dv = ptr<E>(dv), p.dpk = ptr<E>(dpk), p.dpv = ptr<E>(dpv);
     p.nsplit = nsplit, p.prefix_blocks = p_blocks;
     SumArgs<E> a{};

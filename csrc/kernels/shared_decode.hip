@@ -648,7 +648,8 @@ at::Tensor dlgm_latent_attn_decode(const at::Tensor& q, const at::Tensor& cache,
     LatentArgs<E> p{};
     p.q = ptr<E>(q), p.cache = ptr<E>(cache), p.w = ptr<E>(w_kv), p.qa = ptr<E>(qa), p.out = ptr<E>(out);
     p.o = o.data_ptr<float>(), p.ml = ml.data_ptr<float>(), p.lens = lp;
-    p.q_sb = q.stride(0), p.q_sh = q.stride(1), p.c_sb = cache.stride(0), p.c_ss = cache.stride(1), p.w_ss = w_kv.stride(0);
+    p.q_sb = stride_of(q, 0), p.q_sh = stride_of(q, 1), p.w_ss = stride_of(w_kv, 0);
+    p.c_sb = stride_of(cache, 0), p.c_ss = stride_of(cache, 1);
     p.B = B, p.H = H, p.L = L, p.dn = dn, p.dv = dv, p.ns = ns;
     p.scale_log2 = softmax_scale * kLog2e;
     auto run = [&](auto rc) {
@@ -722,11 +723,11 @@ at::Tensor dlgm_prefix_attn_decode(const at::Tensor& q, const at::Tensor& k, con
     PrefixArgs<E> p{};
     p.q = ptr<E>(q), p.k = ptr<E>(k), p.v = ptr<E>(v), p.pk = ptr<E>(prefix_k), p.pv = ptr<E>(prefix_v), p.out = ptr<E>(out);
     p.o = o.data_ptr<float>(), p.ml = ml.data_ptr<float>(), p.lens = lp, p.plens = pp;
-    p.q_sb = q.stride(0), p.q_sh = q.stride(1);
-    p.k_sb = k.stride(0), p.k_ss = k.stride(1), p.k_sh = k.stride(2);
-    p.v_sb = v.stride(0), p.v_ss = v.stride(1), p.v_sh = v.stride(2);
-    p.pk_sb = prefix_k.stride(0), p.pk_ss = prefix_k.stride(1), p.pk_sh = prefix_k.stride(2);
-    p.pv_sb = prefix_v.stride(0), p.pv_ss = prefix_v.stride(1), p.pv_sh = prefix_v.stride(2);
+    p.q_sb = stride_of(q, 0), p.q_sh = stride_of(q, 1);
+    p.k_sb = stride_of(k, 0), p.k_ss = stride_of(k, 1), p.k_sh = stride_of(k, 2);
+    p.v_sb = stride_of(v, 0), p.v_ss = stride_of(v, 1), p.v_sh = stride_of(v, 2);
+    p.pk_sb = stride_of(prefix_k, 0), p.pk_ss = stride_of(prefix_k, 1), p.pk_sh = stride_of(prefix_k, 2);
+    p.pv_sb = stride_of(prefix_v, 0), p.pv_ss = stride_of(prefix_v, 1), p.pv_sh = stride_of(prefix_v, 2);
     p.B = B, p.Hq = Hq, p.Hkv = Hkv, p.L = L, p.P = P, p.G = G, p.n = n;
     p.np = np, p.no = no, p.prw = prw, p.orw = orw, p.prb = prb, p.orb = orb, p.prefix_blocks = pitems * np;
     p.scale_log2 = softmax_scale * kLog2e;

@@ -822,6 +822,28 @@ def test_gradients_that_start_anywhere():
 
 
 @pytest.mark.gpu
+def test_strides_of_dimensions_of_one():
+    """A dimension of one may carry any stride: 1 here, as a permutation of a trailing one gives it."""
+    g = torch.Generator().manual_seed(25)
+    one = lambda t: t.unsqueeze(-1).movedim(-1, 1)  # noqa: E731  [B, H, D] -> [B, 1, H, D] with a row stride of 1
+    x = [rnd(g, 3, h, d, dt=BF, dev=GPU) for h, d in ((2, 96), (2, 128), (2, 64))]
+    kr = rnd(g, 3, 32, dt=BF, dev=GPU)
+    res = []
+    for f in (one, lambda t: t.unsqueeze(1).contiguous()):
+        q, kv, do = (f(t) for t in x)
+        assert f is not one or q.stride(1) == kv.stride(1) == do.stride(1) == f(kr).stride(1) == 1
+        out, lse = ops.latent_attn_fwd(q, kv, f(kr))
+        p = [f(t[..., :64].contiguous()) for t in x]
+        pk = f(x[0][:1, :, :64].contiguous())
+        po, plse = ops.prefix_attn_fwd(*p, pk, pk)
+        lens = torch.tensor([1, 0, 1], dtype=torch.int32, device=GPU)
+        cache, w = f(torch.cat([x[1], x[1], kr.unsqueeze(1).expand(3, 2, 32)], -1)[:, 0].contiguous()), torch.ones(256, 256, dtype=BF, device=GPU) / 16
+        res.append((out, lse, *ops.latent_attn_bwd(do, q, kv, f(kr), out, lse), po, plse, *ops.prefix_attn_bwd(p[2], *p, pk, pk, po, plse),
+                    ops.latent_attention_decode(x[0], cache, lens, w), ops.prefix_attention_decode(p[0][:, 0], p[1], p[2], lens, pk, pk)))
+    assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
+@pytest.mark.gpu
 def test_rows_beyond_32_bit_offsets():
     """Row strides and cache lengths whose byte offsets pass 32 bits."""
     dn, dr, dv = HALF
